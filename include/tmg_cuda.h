@@ -13,7 +13,8 @@
  *    NaN logits; here every such case is a status code.)
  *  - Model-level calls take HOST pointers.  tmg_op_* calls take DEVICE
  *    pointers (16-byte aligned) and run on the context's stream; they return
- *    after the work completes.
+ *    after the work completes, except those whose comment says that they only
+ *    enqueue.
  *  - A context is single-threaded (the reference's `&mut self`): one host
  *    thread per context, one context per GPU.
  *  - Weights are BF16 bit patterns (uint16) laid out [out, in] row-major, as
@@ -372,6 +373,77 @@ int tmg_op_sample(tmg_ctx* ctx, float* logits, int64_t V, int32_t rows, const ui
                   int64_t n_gen, float temperature, int64_t top_k, float top_p, float penalty,
                   const float* uniforms, uint32_t* next, uint32_t* cand_ids, float* cand_probs,
                   int32_t* cutoff);
+
+/* ---------------------------------------------------------------------------
+ * The 4-bit KV cache and token scoring.  No counterpart in the reference.
+ * These calls allocate nothing and only enqueue on the context's stream
+ * (results are ready after tmg_sync; work of the caller's own streams is
+ * ordered against tmg_stream by the caller), so they can be captured into a
+ * CUDA graph.  Positions, lengths and token ids are read on the device: one
+ * that is out of range touches no memory outside its buffers, and tmg_sync
+ * then returns the status that the call's comment names.
+ * ------------------------------------------------------------------------ */
+
+/* Keys and values of n_streams streams in 4 bits, in buffers of the caller
+ * (device pointers, 16-byte aligned).  codes: [n_streams, n_kv, capacity,
+ * head_dim / 2] bytes, element 2i of a row in the low half of byte i.
+ * params: [n_streams, n_kv, capacity, head_dim / g] words, one for each group
+ * of g = min(head_dim, 32) elements: the bf16 minimum m in the high half, the
+ * bf16 step s in the low half; a code stands for m + code * s (one f32
+ * rounding).  head_dim 16, 32, 64 or 128; capacity a multiple of 4; 1 to 1024
+ * streams. */
+typedef struct tmg_kv4 {
+  uint8_t* k_codes;
+  uint32_t* k_params;
+  uint8_t* v_codes;
+  uint32_t* v_params;
+  int32_t n_streams;
+  int32_t n_kv;
+  int32_t head_dim;
+  int64_t capacity;
+} tmg_kv4;
+
+/* Quantise rows of keys (already rotated) and values as they are written:
+ * row t of stream m, at k / v + (m * T + t) * row_ld with head h at h *
+ * head_dim, goes to position pos[m] + t.  count (may be NULL) gives each
+ * stream's number of rows: rows t >= count[m] are padding and neither read
+ * nor written.  Per group: m = the largest bf16 <= its minimum, s = the
+ * smallest bf16 with 15 s >= its maximum - m, code = rint((x - m) / s); so a
+ * value is off by at most s / 2.  A group with a value that is not finite, or
+ * too wide for f32, stands for NaN as a whole.  row_ld a multiple of 4; T at
+ * most the capacity.  A position outside [0, capacity) is skipped
+ * (TMG_ERR_CAPACITY). */
+int tmg_op_kv4_append(tmg_ctx* ctx, const tmg_kv4* kv, const float* k, const float* v,
+                      int64_t row_ld, int64_t T, const int32_t* pos, const int32_t* count);
+/* The same rows read back to f32 (k or v may be NULL): position pos[m] + t of
+ * stream m to row t < count[m] of k and v.  Padding rows and rows whose
+ * position lies outside the cache (TMG_ERR_CAPACITY) are left as they were. */
+int tmg_op_kv4_read(tmg_ctx* ctx, const tmg_kv4* kv, const int32_t* pos, const int32_t* count,
+                    int64_t T, float* k, float* v, int64_t row_ld);
+/* Decode attention over the cache, as tmg_op_attn_decode over f32 rows: for
+ * each stream m one query row q + m * q_ld of n_q heads over its first
+ * lens[m] positions, to out + m * out_ld (a stream of length 0 gets zeros).
+ * At most 16 query heads per kv head.  max_len: a bound of all lengths that
+ * the caller knows (the capacity if none), which sizes the split; a length
+ * outside [0, max_len] is taken as the nearer end (TMG_ERR_INVALID).  ws: at
+ * least the bytes that tmg_op_attn_decode_kv4_ws reports, 16-byte aligned,
+ * contents of no matter before and after; calls that may overlap (two
+ * streams, two graphs in flight) need one each. */
+int tmg_op_attn_decode_kv4_ws(tmg_ctx* ctx, const tmg_kv4* kv, int32_t n_q, int64_t* bytes);
+int tmg_op_attn_decode_kv4(tmg_ctx* ctx, const tmg_kv4* kv, const float* q, int64_t q_ld,
+                           const int32_t* lens, int64_t max_len, int32_t n_q, float* out,
+                           int64_t out_ld, void* ws, int64_t ws_bytes);
+/* Scores of rows of logits (ld floats apart): logprob[r] = the natural log of
+ * the softmax probability of targets[r] (both NULL: none wanted), entropy[r]
+ * (may be NULL) = that distribution's entropy in nats, and the n_top (0 to
+ * 64) most likely tokens in top_ids / top_logprobs [rows, n_top], largest
+ * first, ties to the lower index.  Logits of -inf have probability 0.  A row
+ * with a NaN or +inf, or of -inf only, has no distribution: its logprob,
+ * entropy and top_logprobs are NaN, and its top_ids order NaN as -inf.  A
+ * target outside the vocabulary gives NaN (TMG_ERR_INVALID). */
+int tmg_op_logprobs(tmg_ctx* ctx, const float* logits, int64_t ld, int64_t rows, int64_t V,
+                    const uint32_t* targets, int32_t n_top, float* logprob, float* entropy,
+                    uint32_t* top_ids, float* top_logprobs);
 
 #ifdef __cplusplus
 }

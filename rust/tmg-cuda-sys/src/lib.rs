@@ -50,6 +50,20 @@ pub struct TmgGenParams {
     pub seed: u64,
 }
 
+/// The caller's 4-bit cache buffers (device pointers).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct TmgKv4 {
+    pub k_codes: *mut u8,
+    pub k_params: *mut u32,
+    pub v_codes: *mut u8,
+    pub v_params: *mut u32,
+    pub n_streams: i32,
+    pub n_kv: i32,
+    pub head_dim: i32,
+    pub capacity: i64,
+}
+
 #[repr(C)]
 pub struct TmgCtx {
     _p: [u8; 0],
@@ -164,6 +178,18 @@ unsafe extern "C" {
                          n_gen: i64, temperature: f32, top_k: i64, top_p: f32, penalty: f32,
                          uniforms: *const f32, next: *mut u32, cand_ids: *mut u32,
                          cand_probs: *mut f32, cutoff: *mut i32) -> i32;
+    pub fn tmg_op_kv4_append(ctx: *mut TmgCtx, kv: *const TmgKv4, k: *const f32, v: *const f32,
+                             row_ld: i64, t: i64, pos: *const i32, count: *const i32) -> i32;
+    pub fn tmg_op_kv4_read(ctx: *mut TmgCtx, kv: *const TmgKv4, pos: *const i32, count: *const i32,
+                           t: i64, k: *mut f32, v: *mut f32, row_ld: i64) -> i32;
+    pub fn tmg_op_attn_decode_kv4_ws(ctx: *mut TmgCtx, kv: *const TmgKv4, n_q: i32,
+                                     bytes: *mut i64) -> i32;
+    pub fn tmg_op_attn_decode_kv4(ctx: *mut TmgCtx, kv: *const TmgKv4, q: *const f32, q_ld: i64,
+                                  lens: *const i32, max_len: i64, n_q: i32, out: *mut f32,
+                                  out_ld: i64, ws: *mut c_void, ws_bytes: i64) -> i32;
+    pub fn tmg_op_logprobs(ctx: *mut TmgCtx, logits: *const f32, ld: i64, rows: i64, v: i64,
+                           targets: *const u32, n_top: i32, logprob: *mut f32, entropy: *mut f32,
+                           top_ids: *mut u32, top_logprobs: *mut f32) -> i32;
 }
 
 /// A failed call: its status and `tmg_last_error`'s message.

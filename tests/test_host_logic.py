@@ -162,3 +162,20 @@ def test_entry_points_refuse_bad_arguments_before_any_device_call():
     assert L.tmg_fused_group_init(None, None, uid, 2, 2) == -1
     assert L.tmg_fused_group_init(None, None, uid, 0, 9) == -1
     assert L.tmg_op_attn_prefill(None, None, None, None, 16, 0, 4, 2, 64, None) == -1
+
+
+def test_kv4_and_logprobs_refuse_a_null_context_before_any_device_call():
+    import ctypes
+
+    from tinyminigo_b200._lib import Kv4View, lib
+
+    L = lib()
+    v = Kv4View(256, 256, 256, 256, 1, 1, 64, 64)
+    n = ctypes.c_int64(-1)
+    assert L.tmg_op_kv4_append(None, ctypes.byref(v), 256, 256, 64, 1, 256, None) == -1
+    assert L.tmg_op_kv4_read(None, ctypes.byref(v), 256, None, 1, 256, 256, 64) == -1
+    assert L.tmg_op_attn_decode_kv4_ws(None, ctypes.byref(v), 4, ctypes.byref(n)) == -1
+    assert L.tmg_op_attn_decode_kv4(None, ctypes.byref(v), 256, 256, 256, 64, 4, 256, 256, None,
+                                    0) == -1
+    assert L.tmg_op_logprobs(None, 256, 64, 1, 64, 256, 0, 256, None, None, None) == -1
+    assert n.value == -1

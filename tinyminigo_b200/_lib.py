@@ -54,6 +54,21 @@ class GenParamsC(ctypes.Structure):
     ]
 
 
+class Kv4View(ctypes.Structure):
+    """tmg_kv4: the caller's 4-bit cache buffers (device pointers)."""
+
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("k_params", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("v_params", ctypes.c_void_p),
+        ("n_streams", ctypes.c_int32),
+        ("n_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("capacity", ctypes.c_int64),
+    ]
+
+
 TOKEN_CB = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_uint32, ctypes.c_void_p)
 
 _P = ctypes.c_void_p
@@ -123,6 +138,11 @@ SIGNATURES = {
     "tmg_op_attn_prefill": (_I, [_P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P]),
     "tmg_op_argmax": (_I, [_P, _P, _I64, _I32, _P]),
     "tmg_op_sample": (_I, [_P, _P, _I64, _I32, _P, _I64, _F, _I64, _F, _F, _P, _P, _P, _P, _P]),
+    "tmg_op_kv4_append": (_I, [_P, _P, _P, _P, _I64, _I64, _P, _P]),
+    "tmg_op_kv4_read": (_I, [_P, _P, _P, _P, _I64, _P, _P, _I64]),
+    "tmg_op_attn_decode_kv4_ws": (_I, [_P, _P, _I32, _PI64]),
+    "tmg_op_attn_decode_kv4": (_I, [_P, _P, _P, _I64, _P, _I64, _I32, _P, _I64, _P, _I64]),
+    "tmg_op_logprobs": (_I, [_P, _P, _I64, _I64, _I64, _P, _I32, _P, _P, _P, _P]),
 }
 
 _lib = None

@@ -256,9 +256,14 @@ cudaError_t zero_sync(tmg_ctx* c, void* p, size_t n) {
 }
 
 // The device error word: 1 = NaN logits reached the sampler, 2 = a bounded
-// device-side wait gave up.
+// device-side wait gave up, 3.. = a value read on the device was out of range.
 int err_status(tmg_ctx* c, int32_t w) {
   if (w == 1) return fail(c, TMG_ERR_NAN, "NaN logits reached the sampler");
+  if (w == kErrPosition)
+    return fail(c, TMG_ERR_CAPACITY, "a row's position lies outside the KV cache");
+  if (w == kErrLength)
+    return fail(c, TMG_ERR_INVALID, "a stream's length lies outside [0, max_len]");
+  if (w == kErrToken) return fail(c, TMG_ERR_INVALID, "a token id lies outside the vocabulary");
   return fail(c, TMG_ERR_TIMEOUT, "a bounded device-side wait gave up (pipeline stalled)");
 }
 
@@ -2668,6 +2673,163 @@ int tmg_op_sample(tmg_ctx* c, float* logits, int64_t V, int32_t rows, const uint
   CK(cudaMemcpyAsync(&errw, a.err, 4, cudaMemcpyDeviceToHost, c->stream), "err");
   CK(cudaStreamSynchronize(c->stream), "sample");
   if (errw) return fail(c, TMG_ERR_NAN, "NaN logits reached the sampler");
+  return TMG_OK;
+}
+
+// --- the 4-bit KV cache -------------------------------------------------------
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Checks a caller's view and fills the kernels' form of it; *why says what is wrong.
+static bool kv4_view(const tmg_kv4* v, Kv4* o, std::string* why) {
+  if (!v || !v->k_codes || !v->k_params || !v->v_codes || !v->v_params) {
+    *why = "null cache pointer";
+    return false;
+  }
+  if (v->head_dim != 16 && v->head_dim != 32 && v->head_dim != 64 && v->head_dim != 128) {
+    *why = "head_dim must be 16, 32, 64 or 128";
+    return false;
+  }
+  if (v->n_streams < 1 || v->n_streams > kKv4MaxStreams || v->n_kv < 1 || v->n_kv > 1024) {
+    *why = "1 to 1024 streams and 1 to 1024 kv heads";
+    return false;
+  }
+  if (v->capacity < 4 || v->capacity % 4 || v->capacity > INT32_MAX) {
+    *why = "the capacity must be a positive multiple of 4 below 2^31";
+    return false;
+  }
+  if (!aligned16(v->k_codes) || !aligned16(v->k_params) || !aligned16(v->v_codes) ||
+      !aligned16(v->v_params)) {
+    *why = "cache pointers must be 16-byte aligned";
+    return false;
+  }
+  o->kc = v->k_codes;
+  o->kp = v->k_params;
+  o->vc = v->v_codes;
+  o->vp = v->v_params;
+  o->M = v->n_streams;
+  o->nkv = v->n_kv;
+  o->d = v->head_dim;
+  o->cap = v->capacity;
+  return true;
+}
+
+static int kv4_rows(tmg_ctx* c, const char* name, const tmg_kv4* view, int64_t T, int64_t row_ld,
+                    const void* k, const void* v, const int32_t* pos, Kv4* kv) {
+  if (!c) return TMG_ERR_INVALID;
+  std::string why;
+  if (!kv4_view(view, kv, &why)) return fail(c, TMG_ERR_INVALID, std::string(name) + ": " + why);
+  if (!pos || T < 0 || T > kv->cap)
+    return fail(c, TMG_ERR_INVALID, std::string(name) + ": null positions, or rows beyond the capacity");
+  if (row_ld < int64_t(kv->nkv) * kv->d || row_ld % 4)
+    return fail(c, TMG_ERR_INVALID,
+                std::string(name) + ": row_ld must be a multiple of 4, at least n_kv * head_dim");
+  if (!aligned16(k) || !aligned16(v))
+    return fail(c, TMG_ERR_INVALID, std::string(name) + ": rows must be 16-byte aligned");
+  return TMG_OK;
+}
+
+int tmg_op_kv4_append(tmg_ctx* c, const tmg_kv4* view, const float* k, const float* v,
+                      int64_t row_ld, int64_t T, const int32_t* pos, const int32_t* count) {
+  Kv4 kv;
+  if (!k || !v) return fail(c, TMG_ERR_INVALID, "tmg_op_kv4_append: null rows");
+  const int rc = kv4_rows(c, "tmg_op_kv4_append", view, T, row_ld, k, v, pos, &kv);
+  if (rc) return rc;
+  cudaSetDevice(c->device);
+  CK(launch_kv4_append(kv, k, v, row_ld, T, pos, count, c->d_err, c->stream), "kv4 append");
+  return TMG_OK;
+}
+
+int tmg_op_kv4_read(tmg_ctx* c, const tmg_kv4* view, const int32_t* pos, const int32_t* count,
+                    int64_t T, float* k, float* v, int64_t row_ld) {
+  Kv4 kv;
+  if (!k && !v) return fail(c, TMG_ERR_INVALID, "tmg_op_kv4_read: no output");
+  const int rc = kv4_rows(c, "tmg_op_kv4_read", view, T, row_ld, k, v, pos, &kv);
+  if (rc) return rc;
+  cudaSetDevice(c->device);
+  CK(launch_kv4_read(kv, pos, count, T, k, v, row_ld, c->d_err, c->stream), "kv4 read");
+  return TMG_OK;
+}
+
+static bool attn_kv4_heads(const Kv4& kv, int32_t n_q, std::string* why) {
+  if (n_q >= 1 && n_q % kv.nkv == 0 && n_q / kv.nkv <= 16) return true;
+  *why = "1 to 16 query heads per kv head";
+  return false;
+}
+
+int tmg_op_attn_decode_kv4_ws(tmg_ctx* c, const tmg_kv4* view, int32_t n_q, int64_t* bytes) {
+  Kv4 kv;
+  std::string why;
+  if (!c || !bytes) return fail(c, TMG_ERR_INVALID, "bad argument");
+  if (!kv4_view(view, &kv, &why) || !attn_kv4_heads(kv, n_q, &why))
+    return fail(c, TMG_ERR_INVALID, "tmg_op_attn_decode_kv4_ws: " + why);
+  *bytes = int64_t(attn_kv4_ws(kv, n_q, c->num_sms));
+  return TMG_OK;
+}
+
+int tmg_op_attn_decode_kv4(tmg_ctx* c, const tmg_kv4* view, const float* q, int64_t q_ld,
+                           const int32_t* lens, int64_t max_len, int32_t n_q, float* out,
+                           int64_t out_ld, void* ws, int64_t ws_bytes) {
+  AttnKv4Args a;
+  std::string why;
+  if (!c || !q || !lens || !out) return fail(c, TMG_ERR_INVALID, "bad argument");
+  if (!kv4_view(view, &a.kv, &why) || !attn_kv4_heads(a.kv, n_q, &why))
+    return fail(c, TMG_ERR_INVALID, "tmg_op_attn_decode_kv4: " + why);
+  const int64_t w = int64_t(n_q) * a.kv.d;
+  if (max_len < 0 || max_len > a.kv.cap)
+    return fail(c, TMG_ERR_INVALID, "tmg_op_attn_decode_kv4: max_len lies outside [0, capacity]");
+  if (q_ld < w || q_ld % 4 || out_ld < w || out_ld % 4 || !aligned16(q) || !aligned16(out))
+    return fail(c, TMG_ERR_INVALID,
+                "tmg_op_attn_decode_kv4: rows of q and out must be 16-byte aligned and at least "
+                "n_q * head_dim long");
+  const size_t need = attn_kv4_ws(a.kv, n_q, c->num_sms);
+  if (need && (!ws || !aligned16(ws) || ws_bytes < 0 || size_t(ws_bytes) < need))
+    return fail(c, TMG_ERR_INVALID,
+                "tmg_op_attn_decode_kv4: the workspace must be 16-byte aligned and hold " +
+                    std::to_string(need) + " bytes");
+  cudaSetDevice(c->device);
+  a.q = q;
+  a.q_ld = q_ld;
+  a.lens = lens;
+  a.max_len = max_len;
+  a.nq = n_q;
+  a.scale = 1.0f / sqrtf(float(a.kv.d));
+  a.out = out;
+  a.out_ld = out_ld;
+  a.ws = ws;
+  a.err = c->d_err;
+  CK(launch_attn_kv4(a, c->stream), "attention");
+  return TMG_OK;
+}
+
+// --- scoring --------------------------------------------------------------------
+int tmg_op_logprobs(tmg_ctx* c, const float* logits, int64_t ld, int64_t rows, int64_t V,
+                    const uint32_t* targets, int32_t n_top, float* logprob, float* entropy,
+                    uint32_t* top_ids, float* top_logprobs) {
+  if (!c || !logits || V <= 0 || V > INT32_MAX || ld < V || rows < 0 || rows > INT32_MAX)
+    return fail(c, TMG_ERR_INVALID, "tmg_op_logprobs: bad argument");
+  if ((reinterpret_cast<uintptr_t>(logits) & 3) != 0)
+    return fail(c, TMG_ERR_INVALID, "tmg_op_logprobs: logits must be 4-byte aligned");
+  if (!targets != !logprob)
+    return fail(c, TMG_ERR_INVALID, "tmg_op_logprobs: targets and logprob go together");
+  if (n_top < 0 || n_top > kMaxTopK || n_top > V || (n_top > 0 && (!top_ids || !top_logprobs)))
+    return fail(c, TMG_ERR_INVALID,
+                "tmg_op_logprobs: 0 to 64 alternatives, at most the vocabulary, and room for them");
+  if (!logprob && !entropy && n_top == 0)
+    return fail(c, TMG_ERR_INVALID, "tmg_op_logprobs: no output");
+  cudaSetDevice(c->device);
+  LogprobsArgs a;
+  a.logits = logits;
+  a.ld = ld;
+  a.rows = rows;
+  a.V = V;
+  a.targets = targets;
+  a.logprob = logprob;
+  a.entropy = entropy;
+  a.n_top = n_top;
+  a.top_ids = top_ids;
+  a.top_logprobs = top_logprobs;
+  a.err = c->d_err;
+  CK(launch_logprobs(a, c->stream), "logprobs");
   return TMG_OK;
 }
 

@@ -188,6 +188,49 @@ int attn_decode_noalloc(int device, int num_sms, cudaStream_t s, const float* q,
                         float* out, std::string* why);
 
 // ---------------------------------------------------------------------------
+// The 4-bit KV cache (kv4.cuh: layout and arithmetic).
+// ---------------------------------------------------------------------------
+// Values of the device error word (1: NaN logits, 2: a bounded wait gave up).
+constexpr int kErrPosition = 3;  // a row's position lies outside the cache
+constexpr int kErrLength = 4;    // a stream's length lies outside its bound
+constexpr int kErrToken = 5;     // a token id lies outside the vocabulary
+
+constexpr int kKv4MaxStreams = 1024;
+struct Kv4 {
+  uint8_t* kc = nullptr;   // [M, nkv, cap, d / 2] codes of the keys
+  uint32_t* kp = nullptr;  // [M, nkv, cap, d / min(d, 32)] their parameters
+  uint8_t* vc = nullptr;
+  uint32_t* vp = nullptr;
+  int M = 0, nkv = 0, d = 0;
+  int64_t cap = 0;
+};
+// Quantise rows [M, T] (row_ld floats apart; head h at h * d) of keys and
+// values into positions pos[m].. of each stream; rows t >= count[m] are
+// padding (count null: none is).
+cudaError_t launch_kv4_append(const Kv4& kv, const float* k, const float* v, int64_t row_ld,
+                              int64_t T, const int32_t* pos, const int32_t* count, int32_t* err,
+                              cudaStream_t s);
+// The same rows back to f32 (k or v may be null).
+cudaError_t launch_kv4_read(const Kv4& kv, const int32_t* pos, const int32_t* count, int64_t T,
+                            float* k, float* v, int64_t row_ld, int32_t* err, cudaStream_t s);
+struct AttnKv4Args {
+  Kv4 kv;
+  const float* q = nullptr;  // [M, q_ld]
+  int64_t q_ld = 0;
+  const int32_t* lens = nullptr;  // [M]
+  int64_t max_len = 0;
+  int nq = 0;
+  float scale = 1.f;
+  float* out = nullptr;  // [M, out_ld]
+  int64_t out_ld = 0;
+  void* ws = nullptr;
+  int32_t* err = nullptr;
+};
+cudaError_t launch_attn_kv4(const AttnKv4Args& a, cudaStream_t s);
+// Bytes of workspace that launch_attn_kv4 needs.
+size_t attn_kv4_ws(const Kv4& kv, int nq, int num_sms);
+
+// ---------------------------------------------------------------------------
 // Prefill pieces.
 // ---------------------------------------------------------------------------
 // x[t, :] = embed[tokens[t], :] (bf16 -> f32).
@@ -309,6 +352,22 @@ struct SampleArgs {
   bool record = false;  // finish_step into st
 };
 cudaError_t launch_sample(const SampleArgs& a, cudaStream_t s, bool pdl, int num_sms);
+
+// ---------------------------------------------------------------------------
+// Log probabilities, entropy and top alternatives of rows of logits.
+// ---------------------------------------------------------------------------
+struct LogprobsArgs {
+  const float* logits = nullptr;  // [rows, ld]
+  int64_t ld = 0, rows = 0, V = 0;
+  const uint32_t* targets = nullptr;  // [rows]
+  float* logprob = nullptr;           // [rows], with targets
+  float* entropy = nullptr;           // [rows] or null
+  int n_top = 0;
+  uint32_t* top_ids = nullptr;    // [rows, n_top]
+  float* top_logprobs = nullptr;  // [rows, n_top]
+  int32_t* err = nullptr;
+};
+cudaError_t launch_logprobs(const LogprobsArgs& a, cudaStream_t s);
 int sample_slices(int64_t V, int M, int num_sms);
 
 }  // namespace tmg
