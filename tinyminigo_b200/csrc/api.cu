@@ -1612,6 +1612,7 @@ int tmg_create(int device, const tmg_config* cfg, tmg_ctx** out) {
       run("fused_prepare", fused_prepare()) && run("sample_prepare", sample_prepare()) &&
       run("gemv_i8_prepare", gemv_i8_prepare()) && run("attn_tma_prepare", attn_tma_prepare()) &&
       run("attn_prefill_tc_prepare", attn_prefill_tc_prepare()) &&
+      run("attn_kv4_prepare", attn_kv4_prepare()) &&
       run("error word", dalloc(c->allocs, &c->d_err, 4)) && run("error word", zero_sync(c, c->d_err, 16));
   if (step) {
     g_create_err = std::string("tmg_create: ") + step + ": " + cudaGetErrorString(ce);
@@ -2797,7 +2798,8 @@ int tmg_op_attn_decode_kv4(tmg_ctx* c, const tmg_kv4* view, const float* q, int6
   a.out_ld = out_ld;
   a.ws = ws;
   a.err = c->d_err;
-  CK(launch_attn_kv4(a, c->stream), "attention");
+  a.num_sms = c->num_sms;
+  CK(launch_attn_kv4(a, c->stream, false), "attention");
   return TMG_OK;
 }
 

@@ -2,7 +2,27 @@
 // stream, o = sum_t p_t v_t with p = softmax(q . k_t / sqrt(d)) over the
 // stream's cached positions (the attention of src/model.rs:434-459, whose
 // cache is f32).
+//
+// With k_t = m + s c over each group of 32 elements (codes c, minimum m, step
+// s), q . k_t = sum over groups of s (q . c) + m (sum of q): the products
+// with codes are exact 4-bit integers times q, which the warp matrix
+// instruction takes as f16, and s and m are applied to 32-bit sums.  q is
+// carried as two f16 parts (22 bits; scaled per head by a power of two so
+// that neither part leaves f16's range), the parts as neighbouring columns of
+// one instruction.  Likewise o = sum_t (p_t s_t) (c_t - 8) + sum_t p_t (m_t +
+// 8 s_t): p s in two f16 parts; the codes centred, since the sums of c and
+// of m alone are hundreds of times larger than their sum over a long row.
+//
+// What bounds it is issue slots: at 5 bits an element the memory brings 37
+// elements a clock and SM, so 3.4 lane-instructions an element are all there
+// are.  The matrix instructions are mma.sync (m16n8k16): a key tile meets 4
+// heads' two parts in 8 columns, so tcgen05's 128-row tiles with operands in
+// shared memory would spend more on writing widened codes than they save.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <math.h>
+
+#include <algorithm>
 
 #include "kv4.cuh"
 
@@ -10,101 +30,793 @@ namespace tmg {
 
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;
+constexpr float kLog2e = 1.4426950408889634f;
 
-// One CTA per (query head, stream).  A warp takes 32 positions at a time:
-// a lane scores one of them, then the lanes share the values' columns and
-// walk the 32 positions; online softmax per warp, the warps meet at the end.
+// A warp's tile is TK positions of one head: 64, and 32 for head dim 128, so
+// that a tile is 5 KB in both (2560 and 1536 bytes for the small head dims).
+// NC: column tiles of 4 query heads.
+template <int D, int NC>
+struct Cfg {
+  static constexpr int G = D < 32 ? D : 32, NG = D / G, TK = D == 128 ? 32 : 64;
+  static constexpr int HB = 4 * NC;
+  static constexpr int CODE = TK * D / 2, PAR = TK * NG * 4, STAGE = 2 * (CODE + PAR);
+  static constexpr int NST = NC == 1 ? 2 : 4;       // stages of a warp's ring
+  static constexpr int CTAS = NC == 1 ? 2 : 1;      // CTAs an SM
+  static constexpr int SLOT = HB * (D + 2);         // floats of a partial result
+  static constexpr bool MAP = D >= 64;              // tiles by tensor map (swizzled)
+  static constexpr int SMEM = kWarps * (NST * STAGE + SLOT * 4) + 512;
+};
+
+// 2^x by the SFU's ex2 instruction (relative error about 2^-22; 2^-inf = 0)
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 8x8 transpose of 16-bit elements over the warp (row = lane / 4)
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t y;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+// x's two f16 parts, the upper 11 bits (cut) and the rest, in one word
+__device__ __forceinline__ uint32_t two_parts(float x) {
+  const float h = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
+  return pack_f16(h, x - h);
+}
+// (x & m) | o in one instruction
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t m, uint32_t o) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "r"(m), "r"(o));
+  return y;
+}
+// Two codes in bits 0-3 (or 4-7) of the halves of x to f16 c - 8: 0x6400 | c
+// is 1024 + c, 0x6400 | 16 c is 1024 + 16 c; both steps are exact.
+__device__ __forceinline__ uint32_t centred_lo(uint32_t x) {
+  uint32_t y;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(and_or(x, 0x000f000fu, 0x64006400u)), "r"(0xe408e408u));
+  return y;  // - 1032
+}
+__device__ __forceinline__ uint32_t centred_hi(uint32_t x) {
+  uint32_t y;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;"
+      : "=r"(y)
+      : "r"(and_or(x, 0x00f000f0u, 0x64006400u)), "r"(0x2c002c00u), "r"(0xd480d480u));
+  return y;  // / 16 - 72
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[N]) {
+  if constexpr (N == 4)
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(a));
+  else if constexpr (N == 2)
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
+  else
+    w[0] = lds32(a);
+}
+__device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint64_t* bar, int row,
+                                         int seg) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(seg)
+      : "memory");
+}
+// Byte offset in a tile of 16-byte chunk `c` of row `r` as the tensor map's
+// swizzle lays it out (64-byte rows: chunk ^ (r / 2) % 4; 32-byte rows: chunk
+// ^ (r / 4) % 2), so that 8 rows' words of one chunk lie in 32 banks.
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32) attn_kv4_simple_kernel(const AttnKv4Args a) {
-  constexpr int G = D < 32 ? D : 32, NG = D / G, C = D < 32 ? 1 : D / 32;
-  __shared__ float qs[D];
-  __shared__ float os[kWarps][D], ms[kWarps], ls[kWarps];
-  const int h = blockIdx.x, m = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int kvh = h / (a.nq / a.kv.nkv);
-  int len = a.lens[m];
-  if (len < 0 || len > a.max_len) {
-    if (threadIdx.x == 0 && a.err) atomicCAS(a.err, 0, kErrLength);
-    len = len < 0 ? 0 : int(a.max_len);
-  }
-  for (int i = threadIdx.x; i < D; i += blockDim.x) qs[i] = a.q[int64_t(m) * a.q_ld + h * D + i];
-  __syncthreads();
-  const int64_t row0 = (int64_t(m) * a.kv.nkv + kvh) * a.kv.cap;
-  float mx = -INFINITY, l = 0.f, o[C] = {};
-  for (int t0 = warp * 32; t0 < len; t0 += kWarps * 32) {
-    const int t = t0 + lane;
-    float s = -INFINITY;
-    if (t < len) {
-      const uint32_t* c = reinterpret_cast<const uint32_t*>(a.kv.kc + (row0 + t) * (D / 2));
-      float acc = 0.f;
-      for (int g = 0; g < NG; ++g) {
-        const uint32_t w = a.kv.kp[(row0 + t) * NG + g];
-        const float mn = kv4_min(w), st = kv4_step(w);
-        for (int j = 0; j < G / 8; ++j) {
-          const uint32_t cw = c[g * (G / 8) + j];
+__device__ __forceinline__ uint32_t chunk_off(int r, int c) {
+  if constexpr (D == 128) return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+  if constexpr (D == 64) return r * 32 + ((c ^ ((r >> 2) & 1)) << 4);
+  return r * (D / 2);
+}
+// Row r of a 16-row matrix operand is position key_of(r) of its 16: the
+// value operand's lane t then reads positions t, t + 4, t + 8, t + 12, whose
+// rows lie in different banks.
+__device__ __forceinline__ int key_of(int r) { return (r & 8) + ((r & 7) >> 1) + 4 * (r & 1); }
+
+// The tiles of all streams, in order of (stream, head group, tile).
+struct Plan {
+  AttnKv4Args a;
+  int gh, ngrp;   // query heads a head group, head groups a kv head
+  int VH;         // head groups a stream
+  bool split;     // CTAs take equal runs of tiles (else one head group each)
+  float* part;    // [grid, 2] partial results
+};
+__device__ __forceinline__ int clamped_len(const AttnKv4Args& a, int m) {
+  return min(max(a.lens[m], 0), int(a.max_len));
+}
+// First tile of CTA b of n when `total` tiles are dealt out.
+__device__ __forceinline__ int first_tile(int b, int n, int total) {
+  return int(int64_t(b) * total / n);
+}
+
+struct Cursor {
+  int m, vh, tile, nt;
+};
+
+template <int D, int NC>
+__global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
+    attn_kv4_kernel(const __grid_constant__ CUtensorMap kmap,
+                    const __grid_constant__ CUtensorMap vmap, const Plan pl) {
+  using C = Cfg<D, NC>;
+  constexpr int G = C::G, NG = C::NG, TK = C::TK, KB = TK / 16, HB = C::HB;
+  constexpr int OD = D == 16 ? 2 : 4;  // output dims a lane and group
+  extern __shared__ uint8_t smem[];
+  // 512: the period of the widest swizzle
+  uint8_t* ring = smem + (-smem_u32(smem) & 511u);
+  __shared__ __align__(8) uint64_t full[kWarps][C::NST];
+  __shared__ int pre[kKv4MaxStreams + 1];  // tiles before each stream
+  __shared__ int scan_s[kWarps];
+  __shared__ int slot_seg[2 * kWarps];  // head group of each warp's partials, -1: none
+  const AttnKv4Args& a = pl.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int M = a.kv.M, VH = pl.VH;
+
+  if (tid < kWarps * C::NST) mbar_init(&full[0][0] + tid, 1);
+  if (tid < 2 * kWarps) slot_seg[tid] = -1;
+  mbar_fence_init();
+  pdl_trigger();
+  pdl_wait();
+
+  // tiles before each stream: 4 streams a thread, scanned over the CTA
+  {
+    int n[4], sum = 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            acc = fmaf(qs[g * G + j * 8 + i], fmaf(float((cw >> (4 * i)) & 15u), st, mn), acc);
+    for (int i = 0; i < 4; ++i) {
+      const int m = 4 * tid + i;
+      n[i] = 0;
+      if (m < M) {
+        const int len = a.lens[m];
+        if ((len < 0 || len > a.max_len) && blockIdx.x == 0 && a.err)
+          atomicCAS(a.err, 0, kErrLength);
+        n[i] = (clamped_len(a, m) + TK - 1) / TK * VH;
+      }
+      sum += n[i];
+    }
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) scan_s[warp] = inc;
+    __syncthreads();
+    int at = inc - sum;
+    for (int w = 0; w < warp; ++w) at += scan_s[w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = 4 * tid + i;
+      if (m <= M) pre[m] = at;
+      at += n[i];
+    }
+    if (M == kKv4MaxStreams && tid == kWarps * 32 - 1) pre[M] = at;
+    __syncthreads();
+  }
+
+  // this CTA's tiles [c0, c1), this warp's [w0, w1)
+  int c0, c1;
+  if (pl.split) {
+    const int total = pre[M], n = min(int(gridDim.x), total);
+    if (int(blockIdx.x) >= n) return;
+    c0 = first_tile(blockIdx.x, n, total);
+    c1 = first_tile(blockIdx.x + 1, n, total);
+  } else {
+    const int m = blockIdx.x / VH, nt = (pre[m + 1] - pre[m]) / VH;
+    c0 = pre[m] + blockIdx.x % VH * nt;
+    c1 = c0 + nt;
+    if (nt == 0) {  // an empty stream
+      float* o = a.out + int64_t(m) * a.out_ld;
+      const int vh = blockIdx.x % VH, kvh = vh / pl.ngrp, h0 = vh % pl.ngrp * pl.gh;
+      const int per = a.nq / a.kv.nkv, n = min(pl.gh, per - h0);
+      for (int i = tid; i < n * D; i += blockDim.x) o[(kvh * per + h0) * D + i] = 0.f;
+    }
+  }
+  const int w0 = c0 + (c1 - c0) * warp / kWarps, w1 = c0 + (c1 - c0) * (warp + 1) / kWarps;
+
+  uint8_t* my_ring = ring + warp * C::NST * C::STAGE;
+  float* first_slot = reinterpret_cast<float*>(ring + kWarps * C::NST * C::STAGE) + warp * C::SLOT;
+  float* last_slot = reinterpret_cast<float*>(my_ring);  // once the ring is done with
+  bool alive = true;
+
+  auto locate = [&](int tile) {
+    int lo = 0, hi = M - 1;  // the last stream with pre[m] <= tile
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (pre[mid] <= tile) lo = mid;
+      else hi = mid - 1;
+    }
+    Cursor c;
+    c.m = lo;
+    c.nt = (pre[lo + 1] - pre[lo]) / VH;
+    const int r = tile - pre[lo];
+    c.vh = r / c.nt;
+    c.tile = r - c.vh * c.nt;
+    return c;
+  };
+  auto advance = [&](Cursor& c) {
+    if (++c.tile < c.nt) return;
+    c.tile = 0;
+    if (++c.vh < VH) return;
+    c.vh = 0;
+    do ++c.m;
+    while (c.m < M && pre[c.m + 1] == pre[c.m]);
+    if (c.m < M) c.nt = (pre[c.m + 1] - pre[c.m]) / VH;
+  };
+  // load tile `c` into stage st (one lane)
+  auto load = [&](const Cursor& c, int st) {
+    const int seg = c.m * a.kv.nkv + c.vh / pl.ngrp, row = c.tile * TK;
+    const int n = int(min(int64_t(TK), a.kv.cap - row));  // a multiple of 4
+    uint8_t* s = my_ring + st * C::STAGE;
+    uint64_t* bar = &full[warp][st];
+    const int64_t r0 = int64_t(seg) * a.kv.cap + row;
+    const uint32_t pb = n * NG * 4;
+    if constexpr (C::MAP) {
+      mbar_expect_tx(bar, 2 * (C::CODE + pb));
+      tma_tile(s, &kmap, bar, row, seg);
+      tma_tile(s + C::CODE, &vmap, bar, row, seg);
+    } else {
+      const uint32_t cb = n * (D / 2);
+      mbar_expect_tx(bar, 2 * (cb + pb));
+      bulk_g2s(s, a.kv.kc + r0 * (D / 2), cb, bar);
+      bulk_g2s(s + C::CODE, a.kv.vc + r0 * (D / 2), cb, bar);
+    }
+    bulk_g2s(s + 2 * C::CODE, a.kv.kp + r0 * NG, pb, bar);
+    bulk_g2s(s + 2 * C::CODE + C::PAR, a.kv.vp + r0 * NG, pb, bar);
+  };
+
+  // state of the head group: query head t (+ 4 c) of the lane; its output
+  // dims 4 g .. (2 g .. for head dim 16) of each group
+  float mx[NC], ref[NC], l[NC], cm[NC][NG], o[NC][NG][OD], cq[NC], qs[NC][NG];
+  uint32_t qb[NC][NG][4];
+  auto start = [&](const Cursor& c) {
+    const int per = a.nq / a.kv.nkv, h0 = c.vh % pl.ngrp * pl.gh;
+    const int heads = min(pl.gh, per - h0);
+    const float* q = a.q + int64_t(c.m) * a.q_ld + int64_t(c.vh / pl.ngrp * per + h0) * D;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      // as an operand the lane holds head g / 2 (part g % 2), of each group
+      // the elements that lane t's code words hold
+      const int h = 4 * k + g / 2;
+      constexpr int E = D == 16 ? 4 : 8;
+      float x[NG][E];
+      float big = 0.f;
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+#pragma unroll
+        for (int i = 0; i < E; i += 4) {
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (h < heads) v = *reinterpret_cast<const float4*>(q + h * D + j * G + t * E + i);
+          x[j][i] = v.x, x[j][i + 1] = v.y, x[j][i + 2] = v.z, x[j][i + 3] = v.w;
+          big = fmaxf(big, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        }
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      // a power of two that takes the largest |q| to 2^14 .. 2^15
+      const int e = min(268 - int(__float_as_uint(big) >> 23), 253);
+      const float up = __uint_as_float(uint32_t(e) << 23);
+      const int src = 8 * t;  // a lane that holds head t (+ 4 k) as an operand
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        float sum = 0.f;
+        uint32_t w[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          x[j][i] *= up;
+          sum += x[j][i];
+          // odd codes enter as 16 c
+          w[i] = two_parts(x[j][i] * (i & 1 ? 0.0625f : 1.f));
+          w[i] = g & 1 ? w[i] >> 16 : w[i] & 0xffffu;
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        // codes enter as f16 numbers c * 2^-24
+        qs[k][j] = __shfl_sync(0xffffffffu, sum, src) * 0x1p-24f;
+        constexpr int S = E / 2;  // the two codes of an operand word
+#pragma unroll
+        for (int i = 0; i < S; ++i) qb[k][j][i] = w[i] | (w[i + S] << 16);
+        if constexpr (E == 4) qb[k][j][2] = qb[k][j][3] = 0u;
+      }
+      const float un = __uint_as_float(uint32_t(254 - e) << 23);
+      cq[k] = __shfl_sync(0xffffffffu, un, src) * (a.scale * kLog2e) * 0x1p24f;
+      mx[k] = -INFINITY;
+      ref[k] = -INFINITY;
+      l[k] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        cm[k][j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < OD; ++i) o[k][j][i] = 0.f;
+      }
+    }
+  };
+  // the sums over the lanes that share a head (each had its own positions)
+  auto finish = [&]() {
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+#pragma unroll
+      for (int s = 4; s < 32; s <<= 1) {
+        l[k] += __shfl_xor_sync(0xffffffffu, l[k], s);
+#pragma unroll
+        for (int j = 0; j < NG; ++j) cm[k][j] += __shfl_xor_sync(0xffffffffu, cm[k][j], s);
+      }
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+#pragma unroll
+        for (int i = 0; i < OD; ++i) o[k][j][i] += cm[k][j];
+    }
+  };
+  auto write_out = [&](const Cursor& c) {
+    const int per = a.nq / a.kv.nkv, h0 = c.vh % pl.ngrp * pl.gh;
+    float* out = a.out + int64_t(c.m) * a.out_ld + int64_t(c.vh / pl.ngrp * per + h0) * D;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int h = 4 * k + t;
+      if (h >= min(pl.gh, per - h0)) continue;
+      const float f = 1.0f / l[k];
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+#pragma unroll
+        for (int i = 0; i < OD; ++i) o[k][j][i] *= f;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        float* p = out + h * D + j * G + g * OD;
+        if constexpr (OD == 4)
+          *reinterpret_cast<float4*>(p) = make_float4(o[k][j][0], o[k][j][1], o[k][j][2], o[k][j][3]);
+        else
+          *reinterpret_cast<float2*>(p) = make_float2(o[k][j][0], o[k][j][1]);
+      }
+    }
+  };
+  auto write_slot = [&](float* s) {
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int h = 4 * k + t;
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+#pragma unroll
+        for (int i = 0; i < OD; ++i) s[h * D + j * G + g * OD + i] = o[k][j][i];
+      if (g == 0) s[HB * D + h] = ref[k], s[HB * D + HB + h] = l[k];
+    }
+  };
+
+  if (w0 < w1) {
+    Cursor cur = locate(w0), nxt = cur;
+    for (int i = 0; i < C::NST && w0 + i < w1; ++i) {
+      if (lane == 0) load(nxt, i);
+      advance(nxt);
+    }
+    const int seg_first = cur.m * VH + cur.vh;
+    start(cur);
+    int len = clamped_len(a, cur.m);
+    bool whole = cur.tile == 0;  // the head group began in this warp
+    const int kg = key_of(g);
+    int st = 0;
+    uint32_t phase = 0;
+    for (int T = w0; T < w1; ++T) {
+      if (!mbar_wait(&full[warp][st], phase)) {
+        if (lane == 0 && a.err) atomicCAS(a.err, 0, 2);
+        alive = false;
+        break;
+      }
+      const uint32_t base = smem_u32(my_ring + st * C::STAGE);
+      const int valid = len - cur.tile * TK;  // positions of the tile in the row
+
+      // scores of positions 16 b + 8 i + kg, x[][2 b + i]
+      float x[NC][2 * KB];
+#pragma unroll
+      for (int b = 0; b < KB; ++b) {
+        uint32_t p0[NG], p1[NG];
+        lds_words<NG>(base + 2 * C::CODE + (16 * b + kg) * NG * 4, p0);
+        lds_words<NG>(base + 2 * C::CODE + (16 * b + 8 + kg) * NG * 4, p1);
+#pragma unroll
+        for (int k = 0; k < NC; ++k) x[k][2 * b] = x[k][2 * b + 1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          uint32_t u, v;
+          if constexpr (D == 16) {  // two bytes: one to each half
+            u = lds32(base + chunk_off<D>(16 * b + kg, 0) + (t >> 1) * 4);
+            v = lds32(base + chunk_off<D>(16 * b + 8 + kg, 0) + (t >> 1) * 4);
+            const uint32_t sel = t & 1 ? 0x4342u : 0x4140u;
+            u = __byte_perm(u, 0u, sel);
+            v = __byte_perm(v, 0u, sel);
+          } else {
+            u = lds32(base + chunk_off<D>(16 * b + kg, j) + t * 4);
+            v = lds32(base + chunk_off<D>(16 * b + 8 + kg, j) + t * 4);
+          }
+          const float s0 = kv4_step(p0[j]), m0 = kv4_min(p0[j]);
+          const float s1 = kv4_step(p1[j]), m1 = kv4_min(p1[j]);
+#pragma unroll
+          for (int k = 0; k < NC; ++k) {
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            // codes as f16 numbers below 1: c * 2^-24, 16 c * 2^-24
+            mma_f16(c, u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
+                    qb[k][j][0], qb[k][j][1]);
+            if constexpr (D > 16)
+              mma_f16(c, (u >> 8) & 0x000f000fu, (v >> 8) & 0x000f000fu, (u >> 8) & 0x00f000f0u,
+                      (v >> 8) & 0x00f000f0u, qb[k][j][2], qb[k][j][3]);
+            x[k][2 * b] = fmaf(s0, c[0] + c[1], fmaf(m0, qs[k][j], x[k][2 * b]));
+            x[k][2 * b + 1] = fmaf(s1, c[2] + c[3], fmaf(m1, qs[k][j], x[k][2 * b + 1]));
+          }
         }
       }
-      s = acc * a.scale;
-    }
-    const float nm = fmaxf(mx, warp_max(s));
-    const float ref = nm == -INFINITY ? 0.f : nm;
-    const float al = expf(mx - ref), p = t < len ? expf(s - ref) : 0.f;
-    mx = nm;
-    l = l * al + p;
+      uint32_t pv[2 * KB][NG];  // the values' parameters of the same positions
 #pragma unroll
-    for (int i = 0; i < C; ++i) o[i] *= al;
-    const int n = min(32, len - t0);
-    for (int j = 0; j < n; ++j) {
-      const float pj = __shfl_sync(0xffffffffu, p, j);
-      const int64_t r = row0 + t0 + j;
+      for (int i = 0; i < 2 * KB; ++i)
+        lds_words<NG>(base + 2 * C::CODE + C::PAR + (8 * i + kg) * NG * 4, pv[i]);
+      if (valid < TK) {
 #pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const int e = i * 32 + lane;
-        if (e < D) {
-          const uint32_t w = a.kv.vp[r * NG + e / G];
-          const uint32_t b = a.kv.vc[r * (D / 2) + e / 2];
-          o[i] = fmaf(pj, fmaf(float((b >> (4 * (e & 1))) & 15u), kv4_step(w), kv4_min(w)), o[i]);
+        for (int i = 0; i < 2 * KB; ++i)
+          if (8 * i + kg >= valid) {  // whatever the rows behind the last hold
+#pragma unroll
+            for (int k = 0; k < NC; ++k) x[k][i] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < NG; ++j) pv[i][j] = 0u;
+          }
+      }
+      // a power of two that takes the tile's largest step to 2^14 .. 2^15
+      float big = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2 * KB; ++i)
+#pragma unroll
+        for (int j = 0; j < NG; ++j) big = fmaxf(big, kv4_step(pv[i][j]));
+#pragma unroll
+      for (int s = 4; s < 32; s <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
+      const int e = min(268 - int(__float_as_uint(big) >> 23), 253);
+      const float up = __uint_as_float(uint32_t(e) << 23);
+      const float un = __uint_as_float(uint32_t(254 - e) << 23);
+
+      float p[NC][2 * KB];
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        float top = x[k][0];
+#pragma unroll
+        for (int i = 1; i < 2 * KB; ++i) top = fmaxf(top, x[k][i]);
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+        top = fmaxf(top, mx[k]);
+        mx[k] = top;
+        const float r = top * cq[k], al = ex2_approx(ref[k] - r);
+        ref[k] = r;
+        l[k] *= al;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          cm[k][j] *= al;
+#pragma unroll
+          for (int i = 0; i < OD; ++i) o[k][j][i] *= al;
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * KB; ++i) {
+          p[k][i] = ex2_approx(fmaf(x[k][i], cq[k], -r));
+          l[k] += p[k][i];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        uint32_t pb[NC][2 * KB];
+#pragma unroll
+        for (int i = 0; i < 2 * KB; ++i) {
+          const float s = kv4_step(pv[i][j]), c8 = fmaf(8.f, s, kv4_min(pv[i][j]));
+#pragma unroll
+          for (int k = 0; k < NC; ++k) {
+            cm[k][j] = fmaf(p[k][i], c8, cm[k][j]);
+            pb[k][i] = transpose8(two_parts(p[k][i] * up * s));
+          }
+        }
+        float c[NC][2][4] = {};
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          // the codes of the lane's dims of positions t, t + 4 | t + 8, t + 12
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 16 * b + 4 * i + t;
+            w[i] = lds32(base + C::CODE + chunk_off<D>(r, j) + (D == 16 ? g >> 2 : g >> 1) * 4);
+          }
+          if constexpr (D == 16) {
+            const uint32_t sel = (g & 3) * 0x0101u + 0x0400u;  // byte g of both
+            const uint32_t u = __byte_perm(w[0], w[1], (sel & 0xfu) | ((sel >> 8 & 0xfu) << 8));
+            const uint32_t v = __byte_perm(w[2], w[3], (sel & 0xfu) | ((sel >> 8 & 0xfu) << 8));
+#pragma unroll
+            for (int k = 0; k < NC; ++k)
+              mma_f16(c[k][0], centred_lo(u), centred_hi(u), centred_lo(v), centred_hi(v),
+                      pb[k][2 * b], pb[k][2 * b + 1]);
+          } else {
+            const uint32_t sel = g & 1 ? 0x7632u : 0x5410u;
+            const uint32_t u = __byte_perm(w[0], w[1], sel), v = __byte_perm(w[2], w[3], sel);
+            const uint32_t a0 = centred_lo(u), a1 = centred_hi(u);
+            const uint32_t a2 = centred_lo(v), a3 = centred_hi(v);
+            const uint32_t b0 = centred_lo(u >> 8), b1 = centred_hi(u >> 8);
+            const uint32_t b2 = centred_lo(v >> 8), b3 = centred_hi(v >> 8);
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+              mma_f16(c[k][0], a0, a1, a2, a3, pb[k][2 * b], pb[k][2 * b + 1]);
+              mma_f16(c[k][1], b0, b1, b2, b3, pb[k][2 * b], pb[k][2 * b + 1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
+#pragma unroll
+          for (int i = 0; i < OD; ++i)
+            o[k][j][i] = fmaf(c[k][i / 2][i % 2 * 2] + c[k][i / 2][i % 2 * 2 + 1], un, o[k][j][i]);
+      }
+
+      // the stage is read: fetch the tile NST ahead into it
+      __syncwarp();
+      if (T + C::NST < w1) {
+        if (lane == 0) load(nxt, st);
+        advance(nxt);
+      }
+      if (++st == C::NST) st = 0, phase ^= 1;
+
+      const Cursor was = cur;
+      advance(cur);
+      if (cur.tile == 0 || T + 1 == w1) {  // the head group, or this warp's part of it, ends
+        finish();
+        const int seg = was.m * VH + was.vh;
+        if (whole && cur.tile == 0) {
+          write_out(was);
+        } else {
+          const bool first = seg == seg_first;
+          if (T + 1 == w1) __syncwarp();
+          write_slot(T + 1 == w1 ? last_slot : first_slot);
+          if (lane == 0) slot_seg[2 * warp + (first ? 0 : 1)] = seg;
+          if (lane == 0 && first && T + 1 == w1) slot_seg[2 * warp] = seg | 0x40000000;
+        }
+        if (T + 1 < w1) {
+          start(cur);
+          len = clamped_len(a, cur.m);
+          whole = true;
         }
       }
     }
+    if (!alive)  // let the copies in flight land before the CTA leaves
+      for (int i = 0; i < C::NST; ++i) mbar_wait(&full[warp][i], i < st ? phase ^ 1 : phase);
   }
-  l = warp_sum(l);
-  if (lane == 0) ms[warp] = mx, ls[warp] = l;
-#pragma unroll
-  for (int i = 0; i < C; ++i)
-    if (i * 32 + lane < D) os[warp][i * 32 + lane] = o[i];
   __syncthreads();
-  float M = -INFINITY;
-  for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ms[w]);
-  const float ref = M == -INFINITY ? 0.f : M;
-  for (int e = threadIdx.x; e < D; e += blockDim.x) {
-    float tot = 0.f, acc = 0.f;
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = expf(ms[w] - ref);
-      tot += ls[w] * f;
-      acc = fmaf(os[w][e], f, acc);
+
+  // Partial results of neighbouring warps with the same head group meet: runs
+  // of slots in warp order.  A run that is the whole head group is written
+  // out, another goes to the CTA's workspace slot (0: it holds the CTA's first
+  // tile, else 1).
+  int run = -1;
+  for (int i = 0, prev = -1; i < 2 * kWarps; ++i) {
+    const int seg = slot_seg[i];
+    if (seg < 0) continue;
+    const int id = seg & 0x3fffffff;
+    const bool head = id != prev;
+    prev = id;
+    if (head) ++run;
+    if (!head || run % kWarps != warp) continue;
+    // this warp joins the run that starts at slot i
+    auto slot = [&](int s) {
+      const bool last = (s & 1) || (slot_seg[s] & 0x40000000);
+      return last ? reinterpret_cast<const float*>(ring + (s >> 1) * C::NST * C::STAGE)
+                  : reinterpret_cast<const float*>(ring + kWarps * C::NST * C::STAGE) +
+                        (s >> 1) * C::SLOT;
+    };
+    int end = i;
+    for (int s = i; s < 2 * kWarps; ++s) {
+      if (slot_seg[s] < 0) continue;
+      if ((slot_seg[s] & 0x3fffffff) != id) break;
+      end = s;
     }
-    a.out[int64_t(m) * a.out_ld + h * D + e] = len > 0 ? acc / tot : 0.f;
+    const int m = id / VH, vh = id % VH, nt = (pre[m + 1] - pre[m]) / VH;
+    const int s0 = pre[m] + vh * nt;
+    const bool complete = s0 >= c0 && s0 + nt <= c1;
+    const int per = a.nq / a.kv.nkv, h0 = vh % pl.ngrp * pl.gh, heads = min(pl.gh, per - h0);
+    float* out = a.out + int64_t(m) * a.out_ld + int64_t(vh / pl.ngrp * per + h0) * D;
+    float* part = pl.part + (int64_t(blockIdx.x) * 2 + (s0 <= c0 ? 0 : 1)) * C::SLOT;
+    for (int h = 0; h < heads; ++h) {
+      float r = -INFINITY;
+      for (int s = i; s <= end; ++s)
+        if (slot_seg[s] >= 0) r = fmaxf(r, slot(s)[HB * D + h]);
+      float ls = 0.f, acc[(D + 31) / 32] = {};
+      for (int s = i; s <= end; ++s) {
+        if (slot_seg[s] < 0) continue;
+        const float* p = slot(s);
+        const float f = ex2_approx(p[HB * D + h] - r);
+        ls = fmaf(p[HB * D + HB + h], f, ls);
+#pragma unroll
+        for (int q = 0; q < (D + 31) / 32; ++q)
+          if (q * 32 + lane < D) acc[q] = fmaf(p[h * D + q * 32 + lane], f, acc[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < (D + 31) / 32; ++q)
+        if (q * 32 + lane < D) {
+          if (complete) out[h * D + q * 32 + lane] = acc[q] / ls;
+          else part[h * D + q * 32 + lane] = acc[q];
+        }
+      if (!complete && lane == 0) part[HB * D + h] = r, part[HB * D + HB + h] = ls;
+    }
   }
+}
+
+// The head groups that several CTAs shared, joined from the workspace (one
+// CTA each), and zeros for empty streams.
+template <int D, int NC>
+__global__ void __launch_bounds__(D * 4) attn_kv4_join_kernel(const Plan pl, int grid) {
+  using C = Cfg<D, NC>;
+  __shared__ int sums[2][D * 4 / 32];
+  const AttnKv4Args& a = pl.a;
+  const int VH = pl.VH, m = blockIdx.x / VH, vh = blockIdx.x % VH, tid = threadIdx.x;
+  pdl_trigger();
+  pdl_wait();
+  int before = 0, total = 0;
+  for (int i = tid; i < a.kv.M; i += blockDim.x) {
+    const int n = (clamped_len(a, i) + C::TK - 1) / C::TK * VH;
+    total += n;
+    if (i < m) before += n;
+  }
+  before = __reduce_add_sync(0xffffffffu, before);
+  total = __reduce_add_sync(0xffffffffu, total);
+  if (tid % 32 == 0) sums[0][tid / 32] = before, sums[1][tid / 32] = total;
+  __syncthreads();
+  before = total = 0;
+  for (int w = 0; w < D * 4 / 32; ++w) before += sums[0][w], total += sums[1][w];
+  const int nt = (clamped_len(a, m) + C::TK - 1) / C::TK;
+  const int per = a.nq / a.kv.nkv, h0 = vh % pl.ngrp * pl.gh, heads = min(pl.gh, per - h0);
+  float* out = a.out + int64_t(m) * a.out_ld + int64_t(vh / pl.ngrp * per + h0) * D;
+  if (nt == 0) {
+    for (int i = tid; i < heads * D; i += blockDim.x) out[i] = 0.f;
+    return;
+  }
+  const int s0 = before + vh * nt, s1 = s0 + nt;
+  grid = min(grid, total);  // every CTA that has a run has a tile
+  // the CTA whose run holds tile T
+  auto owner = [&](int T) { return int((int64_t(T + 1) * grid - 1) / total); };
+  const int b0 = owner(s0), b1 = owner(s1 - 1);
+  if (b0 == b1) return;
+  auto slot = [&](int b) {
+    return pl.part + (int64_t(b) * 2 + (s0 <= first_tile(b, grid, total) ? 0 : 1)) * C::SLOT;
+  };
+  for (int i = tid; i < heads * D; i += blockDim.x) {
+    const int h = i / D;
+    float r = -INFINITY;
+    for (int b = b0; b <= b1; ++b) r = fmaxf(r, __ldcg(slot(b) + C::HB * D + h));
+    float ls = 0.f, acc = 0.f;
+    for (int b = b0; b <= b1; ++b) {
+      const float* p = slot(b);
+      const float f = ex2_approx(__ldcg(p + C::HB * D + h) - r);
+      ls = fmaf(__ldcg(p + C::HB * D + C::HB + h), f, ls);
+      acc = fmaf(__ldcg(p + i), f, acc);
+    }
+    out[i] = acc / ls;
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
+  static const auto fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  return fn;
+}
+
+// A map over the codes [M * nkv, cap, d / 2] with a box of `rows` rows; a
+// box reaching behind a head's last row reads zeros there.
+bool code_map(CUtensorMap* map, const uint8_t* base, const Kv4& kv, int rows) {
+  auto fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint64_t row = kv.d / 2;
+  const cuuint64_t dims[3] = {row, cuuint64_t(kv.cap), cuuint64_t(kv.M) * kv.nkv};
+  const cuuint64_t strides[2] = {row, row * kv.cap};
+  const cuuint32_t box[3] = {cuuint32_t(row), cuuint32_t(rows), 1}, estr[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(base), dims, strides, box,
+            estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            kv.d == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename K, typename... A>
+cudaError_t launch(K kern, int grid, int threads, int smem, cudaStream_t s, bool pdl, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// Query heads a head group: at most 8 (two column tiles).
+int head_groups(int per) { return (per + 7) / 8; }
+
+template <int D, int NC>
+cudaError_t run(const AttnKv4Args& a, cudaStream_t s, bool pdl) {
+  using C = Cfg<D, NC>;
+  Plan pl;
+  const int per = a.nq / a.kv.nkv;
+  pl.a = a;
+  pl.ngrp = head_groups(per);
+  pl.gh = (per + pl.ngrp - 1) / pl.ngrp;
+  pl.VH = a.kv.nkv * pl.ngrp;
+  pl.part = static_cast<float*>(a.ws);
+  CUtensorMap km = {}, vm = {};
+  if (C::MAP && (!code_map(&km, a.kv.kc, a.kv, C::TK) || !code_map(&vm, a.kv.vc, a.kv, C::TK)))
+    return cudaErrorInvalidValue;
+  const int64_t groups = int64_t(a.kv.M) * pl.VH;
+  pl.split = a.max_len > 16 * C::TK;
+  const int grid = pl.split ? a.num_sms * C::CTAS : int(groups);
+  TMG_CUDA_TRY(launch(attn_kv4_kernel<D, NC>, grid, kWarps * 32, C::SMEM, s, pdl, km, vm, pl));
+  if (!pl.split) return cudaSuccess;
+  return launch(attn_kv4_join_kernel<D, NC>, int(groups), D * 4, 0, s, true, pl, grid);
+}
+
+template <int D, int NC>
+cudaError_t prepare() {
+  TMG_CUDA_TRY(set_carveout(attn_kv4_kernel<D, NC>, Cfg<D, NC>::SMEM));
+  return set_carveout(attn_kv4_join_kernel<D, NC>);
+}
+
+int column_tiles(int per) {
+  const int n = head_groups(per);
+  return (per + n - 1) / n > 4 ? 2 : 1;
 }
 
 }  // namespace
 
-size_t attn_kv4_ws(const Kv4&, int, int) { return 0; }
+cudaError_t attn_kv4_prepare() {
+  TMG_CUDA_TRY((prepare<16, 1>()));
+  TMG_CUDA_TRY((prepare<16, 2>()));
+  TMG_CUDA_TRY((prepare<32, 1>()));
+  TMG_CUDA_TRY((prepare<32, 2>()));
+  TMG_CUDA_TRY((prepare<64, 1>()));
+  TMG_CUDA_TRY((prepare<64, 2>()));
+  TMG_CUDA_TRY((prepare<128, 1>()));
+  return prepare<128, 2>();
+}
 
-cudaError_t launch_attn_kv4(const AttnKv4Args& a, cudaStream_t s) {
-  const dim3 grid(a.nq, a.kv.M);
-  switch (a.kv.d) {
-    case 16: attn_kv4_simple_kernel<16><<<grid, kWarps * 32, 0, s>>>(a); break;
-    case 32: attn_kv4_simple_kernel<32><<<grid, kWarps * 32, 0, s>>>(a); break;
-    case 64: attn_kv4_simple_kernel<64><<<grid, kWarps * 32, 0, s>>>(a); break;
-    case 128: attn_kv4_simple_kernel<128><<<grid, kWarps * 32, 0, s>>>(a); break;
-    default: return cudaErrorInvalidValue;
+size_t attn_kv4_ws(const Kv4& kv, int nq, int num_sms) {
+  const int nc = column_tiles(nq / kv.nkv);
+  // Cfg's CTAS and SLOT
+  return size_t(num_sms) * (nc == 1 ? 2 : 1) * 2 * (4 * nc) * (kv.d + 2) * 4;
+}
+
+cudaError_t launch_attn_kv4(const AttnKv4Args& a, cudaStream_t s, bool pdl) {
+  const int nc = column_tiles(a.nq / a.kv.nkv);
+  switch (a.kv.d * 10 + nc) {
+    case 161: return run<16, 1>(a, s, pdl);
+    case 162: return run<16, 2>(a, s, pdl);
+    case 321: return run<32, 1>(a, s, pdl);
+    case 322: return run<32, 2>(a, s, pdl);
+    case 641: return run<64, 1>(a, s, pdl);
+    case 642: return run<64, 2>(a, s, pdl);
+    case 1281: return run<128, 1>(a, s, pdl);
+    case 1282: return run<128, 2>(a, s, pdl);
   }
-  return cudaGetLastError();
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace tmg

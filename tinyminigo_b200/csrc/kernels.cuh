@@ -225,8 +225,10 @@ struct AttnKv4Args {
   int64_t out_ld = 0;
   void* ws = nullptr;
   int32_t* err = nullptr;
+  int num_sms = 148;
 };
-cudaError_t launch_attn_kv4(const AttnKv4Args& a, cudaStream_t s);
+cudaError_t launch_attn_kv4(const AttnKv4Args& a, cudaStream_t s, bool pdl);
+cudaError_t attn_kv4_prepare();
 // Bytes of workspace that launch_attn_kv4 needs.
 size_t attn_kv4_ws(const Kv4& kv, int nq, int num_sms);
 
