@@ -43,7 +43,7 @@ struct Cfg {
   static constexpr int CODE = TK * D / 2, PAR = TK * NG * 4, STAGE = 2 * (CODE + PAR);
   static constexpr int NST = NC == 1 ? 2 : 4;       // stages of a warp's ring
   static constexpr int CTAS = NC == 1 ? 2 : 1;      // CTAs an SM
-  static constexpr int SLOT = HB * (D + 2);         // floats of a partial result
+  static constexpr int SLOT = HB * (D + 2);         // floats of a partial result (a multiple of 4)
   static constexpr bool MAP = D >= 64;              // tiles by tensor map (swizzled)
   static constexpr int SMEM = kWarps * (NST * STAGE + SLOT * 4) + 512;
 };
@@ -122,6 +122,9 @@ __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(seg)
       : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 // Byte offset in a tile of 16-byte chunk `c` of row `r` as the tensor map's
 // swizzle lays it out (64-byte rows: chunk ^ (r / 2) % 4; 32-byte rows: chunk
 // ^ (r / 4) % 2), so that 8 rows' words of one chunk lie in 32 banks.
@@ -139,7 +142,7 @@ __device__ __forceinline__ int key_of(int r) { return (r & 8) + ((r & 7) >> 1) +
 // The tiles of all streams, in order of (stream, head group, tile).
 struct Plan {
   AttnKv4Args a;
-  int gh, ngrp;   // query heads a head group, head groups a kv head
+  int gh, gsh;    // query heads a head group; log2 of a kv head's head groups
   int VH;         // head groups a stream
   bool split;     // CTAs take equal runs of tiles (else one head group each)
   float* part;    // [grid, 2] partial results
@@ -152,6 +155,7 @@ __device__ __forceinline__ int first_tile(int b, int n, int total) {
   return int(int64_t(b) * total / n);
 }
 
+// A head group and the tile that a warp has reached in it.
 struct Cursor {
   int m, vh, tile, nt;
 };
@@ -176,23 +180,29 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
 
   if (tid < kWarps * C::NST) mbar_init(&full[0][0] + tid, 1);
   if (tid < 2 * kWarps) slot_seg[tid] = -1;
+  if constexpr (C::MAP)
+    if (tid == 0) {
+      prefetch_map(&kmap);
+      prefetch_map(&vmap);
+    }
   mbar_fence_init();
   pdl_trigger();
   pdl_wait();
 
-  // tiles before each stream: 4 streams a thread, scanned over the CTA
-  {
+  auto checked_tiles = [&](int m) {
+    const int len = a.lens[m];
+    if ((len < 0 || len > a.max_len) && a.err) atomicCAS(a.err, 0, kErrLength);
+    return (clamped_len(a, m) + TK - 1) / TK;
+  };
+  // this CTA's tiles [c0, c1)
+  int c0, c1;
+  if (pl.split) {
+    // tiles (of one head group) before each stream: 4 streams a thread,
+    // scanned over the CTA
     int n[4], sum = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int m = 4 * tid + i;
-      n[i] = 0;
-      if (m < M) {
-        const int len = a.lens[m];
-        if ((len < 0 || len > a.max_len) && blockIdx.x == 0 && a.err)
-          atomicCAS(a.err, 0, kErrLength);
-        n[i] = (clamped_len(a, m) + TK - 1) / TK * VH;
-      }
+      n[i] = 4 * tid + i < M ? checked_tiles(4 * tid + i) : 0;
       sum += n[i];
     }
     int inc = sum;
@@ -207,31 +217,26 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
     for (int w = 0; w < warp; ++w) at += scan_s[w];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int m = 4 * tid + i;
-      if (m <= M) pre[m] = at;
+      if (4 * tid + i <= M) pre[4 * tid + i] = at;
       at += n[i];
     }
     if (M == kKv4MaxStreams && tid == kWarps * 32 - 1) pre[M] = at;
     __syncthreads();
-  }
-
-  // this CTA's tiles [c0, c1), this warp's [w0, w1)
-  int c0, c1;
-  if (pl.split) {
-    const int total = pre[M], n = min(int(gridDim.x), total);
-    if (int(blockIdx.x) >= n) return;
-    c0 = first_tile(blockIdx.x, n, total);
-    c1 = first_tile(blockIdx.x + 1, n, total);
-  } else {
-    const int m = blockIdx.x / VH, nt = (pre[m + 1] - pre[m]) / VH;
-    c0 = pre[m] + blockIdx.x % VH * nt;
-    c1 = c0 + nt;
-    if (nt == 0) {  // an empty stream
-      float* o = a.out + int64_t(m) * a.out_ld;
-      const int vh = blockIdx.x % VH, kvh = vh / pl.ngrp, h0 = vh % pl.ngrp * pl.gh;
-      const int per = a.nq / a.kv.nkv, n = min(pl.gh, per - h0);
-      for (int i = tid; i < n * D; i += blockDim.x) o[(kvh * per + h0) * D + i] = 0.f;
+    const int total = pre[M] * VH, ctas = min(int(gridDim.x), total);
+    if (int(blockIdx.x) >= ctas) return;
+    c0 = first_tile(blockIdx.x, ctas, total);
+    c1 = first_tile(blockIdx.x + 1, ctas, total);
+  } else {  // one head group: its tiles count from 0
+    const int m = blockIdx.x / VH, vh = blockIdx.x - m * VH;
+    c0 = 0;
+    c1 = checked_tiles(m);
+    if (c1 == 0) {  // an empty stream
+      const int per = a.nq / a.kv.nkv, h0 = (vh & ((1 << pl.gsh) - 1)) * pl.gh;
+      float* o = a.out + int64_t(m) * a.out_ld + int64_t((vh >> pl.gsh) * per + h0) * D;
+      for (int i = tid; i < min(pl.gh, per - h0) * D; i += blockDim.x) o[i] = 0.f;
+      return;
     }
+    __syncthreads();  // the mbarriers and slots above
   }
   const int w0 = c0 + (c1 - c0) * warp / kWarps, w1 = c0 + (c1 - c0) * (warp + 1) / kWarps;
 
@@ -241,16 +246,23 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
   bool alive = true;
 
   auto locate = [&](int tile) {
-    int lo = 0, hi = M - 1;  // the last stream with pre[m] <= tile
+    Cursor c;
+    if (!pl.split) {
+      c.m = blockIdx.x / VH;
+      c.vh = blockIdx.x - c.m * VH;
+      c.tile = tile;
+      c.nt = c1;
+      return c;
+    }
+    int lo = 0, hi = M - 1;  // the last stream with pre[m] VH <= tile
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (pre[mid] <= tile) lo = mid;
+      if (pre[mid] * VH <= tile) lo = mid;
       else hi = mid - 1;
     }
-    Cursor c;
     c.m = lo;
-    c.nt = (pre[lo + 1] - pre[lo]) / VH;
-    const int r = tile - pre[lo];
+    c.nt = pre[lo + 1] - pre[lo];
+    const int r = tile - pre[lo] * VH;
     c.vh = r / c.nt;
     c.tile = r - c.vh * c.nt;
     return c;
@@ -258,19 +270,22 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
   auto advance = [&](Cursor& c) {
     if (++c.tile < c.nt) return;
     c.tile = 0;
-    if (++c.vh < VH) return;
+    if (!pl.split || ++c.vh < VH) return;
     c.vh = 0;
     do ++c.m;
     while (c.m < M && pre[c.m + 1] == pre[c.m]);
-    if (c.m < M) c.nt = (pre[c.m + 1] - pre[c.m]) / VH;
+    if (c.m < M) c.nt = pre[c.m + 1] - pre[c.m];
   };
+  // the query heads of head group vh: the first and their number
+  const int per = a.nq / a.kv.nkv, gmask = (1 << pl.gsh) - 1;
+  auto first_head = [&](int vh) { return (vh >> pl.gsh) * per + (vh & gmask) * pl.gh; };
+  auto n_heads = [&](int vh) { return min(pl.gh, per - (vh & gmask) * pl.gh); };
   // load tile `c` into stage st (one lane)
-  auto load = [&](const Cursor& c, int st) {
-    const int seg = c.m * a.kv.nkv + c.vh / pl.ngrp, row = c.tile * TK;
-    const int n = int(min(int64_t(TK), a.kv.cap - row));  // a multiple of 4
+  auto load = [&](const Cursor& c, int64_t par, int seg, int st) {
+    const int row = c.tile * TK;
+    const int n = min(TK, int(a.kv.cap) - row);  // a multiple of 4
     uint8_t* s = my_ring + st * C::STAGE;
     uint64_t* bar = &full[warp][st];
-    const int64_t r0 = int64_t(seg) * a.kv.cap + row;
     const uint32_t pb = n * NG * 4;
     if constexpr (C::MAP) {
       mbar_expect_tx(bar, 2 * (C::CODE + pb));
@@ -279,21 +294,25 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
     } else {
       const uint32_t cb = n * (D / 2);
       mbar_expect_tx(bar, 2 * (cb + pb));
-      bulk_g2s(s, a.kv.kc + r0 * (D / 2), cb, bar);
-      bulk_g2s(s + C::CODE, a.kv.vc + r0 * (D / 2), cb, bar);
+      bulk_g2s(s, a.kv.kc + par * (G / 2), cb, bar);
+      bulk_g2s(s + C::CODE, a.kv.vc + par * (G / 2), cb, bar);
     }
-    bulk_g2s(s + 2 * C::CODE, a.kv.kp + r0 * NG, pb, bar);
-    bulk_g2s(s + 2 * C::CODE + C::PAR, a.kv.vp + r0 * NG, pb, bar);
+    bulk_g2s(s + 2 * C::CODE, a.kv.kp + par, pb, bar);
+    bulk_g2s(s + 2 * C::CODE + C::PAR, a.kv.vp + par, pb, bar);
+  };
+  // cache head and index of the first parameter word of tile `c`
+  auto head_of = [&](const Cursor& c) { return c.m * a.kv.nkv + (c.vh >> pl.gsh); };
+  auto par_of = [&](const Cursor& c) {
+    return (int64_t(head_of(c)) * a.kv.cap + c.tile * TK) * NG;
   };
 
   // state of the head group: query head t (+ 4 c) of the lane; its output
   // dims 4 g .. (2 g .. for head dim 16) of each group
-  float mx[NC], ref[NC], l[NC], cm[NC][NG], o[NC][NG][OD], cq[NC], qs[NC][NG];
+  float ref[NC], l[NC], cm[NC][NG], o[NC][NG][OD], cq[NC], qs[NC][NG];
   uint32_t qb[NC][NG][4];
   auto start = [&](const Cursor& c) {
-    const int per = a.nq / a.kv.nkv, h0 = c.vh % pl.ngrp * pl.gh;
-    const int heads = min(pl.gh, per - h0);
-    const float* q = a.q + int64_t(c.m) * a.q_ld + int64_t(c.vh / pl.ngrp * per + h0) * D;
+    const int heads = n_heads(c.vh);
+    const float* q = a.q + int64_t(c.m) * a.q_ld + int64_t(first_head(c.vh)) * D;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       // as an operand the lane holds head g / 2 (part g % 2), of each group
@@ -340,7 +359,6 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
       }
       const float un = __uint_as_float(uint32_t(254 - e) << 23);
       cq[k] = __shfl_sync(0xffffffffu, un, src) * (a.scale * kLog2e) * 0x1p24f;
-      mx[k] = -INFINITY;
       ref[k] = -INFINITY;
       l[k] = 0.f;
 #pragma unroll
@@ -368,12 +386,12 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
     }
   };
   auto write_out = [&](const Cursor& c) {
-    const int per = a.nq / a.kv.nkv, h0 = c.vh % pl.ngrp * pl.gh;
-    float* out = a.out + int64_t(c.m) * a.out_ld + int64_t(c.vh / pl.ngrp * per + h0) * D;
+    const int heads = n_heads(c.vh);
+    float* out = a.out + int64_t(c.m) * a.out_ld + int64_t(first_head(c.vh)) * D;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int h = 4 * k + t;
-      if (h >= min(pl.gh, per - h0)) continue;
+      if (h >= heads) continue;
       const float f = 1.0f / l[k];
 #pragma unroll
       for (int j = 0; j < NG; ++j)
@@ -403,10 +421,18 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
 
   if (w0 < w1) {
     Cursor cur = locate(w0), nxt = cur;
-    for (int i = 0; i < C::NST && w0 + i < w1; ++i) {
-      if (lane == 0) load(nxt, i);
+    int64_t nxt_par = par_of(nxt);
+    int nxt_head = head_of(nxt);
+    auto fetch = [&](int st) {
+      if (lane == 0) load(nxt, nxt_par, nxt_head, st);
       advance(nxt);
-    }
+      nxt_par += TK * NG;
+      if (nxt.tile == 0) {
+        nxt_par = par_of(nxt);
+        nxt_head = head_of(nxt);
+      }
+    };
+    for (int i = 0; i < C::NST && w0 + i < w1; ++i) fetch(i);
     const int seg_first = cur.m * VH + cur.vh;
     start(cur);
     int len = clamped_len(a, cur.m);
@@ -475,43 +501,64 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
             for (int j = 0; j < NG; ++j) pv[i][j] = 0u;
           }
       }
-      // a power of two that takes the tile's largest step to 2^14 .. 2^15
-      float big = 0.f;
+      // the tile's largest step, as the lower halves of the words (a NaN step
+      // does not count)
+      uint32_t big = 0;
 #pragma unroll
       for (int i = 0; i < 2 * KB; ++i)
 #pragma unroll
-        for (int j = 0; j < NG; ++j) big = fmaxf(big, kv4_step(pv[i][j]));
+        for (int j = 0; j < NG; j += 2)
+          big = __vimax3_u16x2(big, pv[i][j], pv[i][j + 1 < NG ? j + 1 : j]);
+      big = __reduce_max_sync(0xffffffffu, big & 0xffffu);
+      if (big >= 0x7f80u) {
+        float f = 0.f;
 #pragma unroll
-      for (int s = 4; s < 32; s <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
-      const int e = min(268 - int(__float_as_uint(big) >> 23), 253);
-      const float up = __uint_as_float(uint32_t(e) << 23);
-      const float un = __uint_as_float(uint32_t(254 - e) << 23);
+        for (int i = 0; i < 2 * KB; ++i)
+#pragma unroll
+          for (int j = 0; j < NG; ++j) f = fmaxf(f, kv4_step(pv[i][j]));
+        big = __reduce_max_sync(0xffffffffu, __float_as_uint(f)) >> 16;
+      }
 
+      // p = 2^(x cq - ref), where ref is a bound of the row's exponents so far
+      // plus one of its steps' less 12: p times a step stays in f16's range,
+      // with 2^4 to spare before ref has to grow.  Steps below 2^-90 count as
+      // that, so that sums of p stay in f32's range.
+      const float step = fmaxf(__uint_as_float(big << 16), 0x1p-90f);
       float p[NC][2 * KB];
+      float top[NC];
+      bool grow = false;
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
-        float top = x[k][0];
+        top[k] = x[k][0];
 #pragma unroll
-        for (int i = 1; i < 2 * KB; ++i) top = fmaxf(top, x[k][i]);
+        for (int i = 1; i < 2 * KB; ++i) top[k] = fmaxf(top[k], x[k][i]);
+        grow |= !(ex2_approx(fmaf(top[k], cq[k], -ref[k])) * step <= 65000.f);
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+        const float room = 12.f - float(int(__float_as_uint(step) >> 23) - 126);
 #pragma unroll
-        for (int s = 4; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-        top = fmaxf(top, mx[k]);
-        mx[k] = top;
-        const float r = top * cq[k], al = ex2_approx(ref[k] - r);
-        ref[k] = r;
-        l[k] *= al;
+        for (int k = 0; k < NC; ++k) {
 #pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          cm[k][j] *= al;
+          for (int s = 4; s < 32; s <<= 1)
+            top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], s));
+          const float r = fmaxf(ref[k], fmaf(top[k], cq[k], -room)), al = ex2_approx(ref[k] - r);
+          ref[k] = r;
+          l[k] *= al;
 #pragma unroll
-          for (int i = 0; i < OD; ++i) o[k][j][i] *= al;
-        }
+          for (int j = 0; j < NG; ++j) {
+            cm[k][j] *= al;
 #pragma unroll
-        for (int i = 0; i < 2 * KB; ++i) {
-          p[k][i] = ex2_approx(fmaf(x[k][i], cq[k], -r));
-          l[k] += p[k][i];
+            for (int i = 0; i < OD; ++i) o[k][j][i] *= al;
+          }
         }
       }
+#pragma unroll
+      for (int k = 0; k < NC; ++k)
+#pragma unroll
+        for (int i = 0; i < 2 * KB; ++i) {
+          p[k][i] = ex2_approx(fmaf(x[k][i], cq[k], -ref[k]));
+          l[k] += p[k][i];
+        }
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         uint32_t pb[NC][2 * KB];
@@ -521,7 +568,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
 #pragma unroll
           for (int k = 0; k < NC; ++k) {
             cm[k][j] = fmaf(p[k][i], c8, cm[k][j]);
-            pb[k][i] = transpose8(two_parts(p[k][i] * up * s));
+            pb[k][i] = transpose8(two_parts(p[k][i] * s));
           }
         }
         float c[NC][2][4] = {};
@@ -560,15 +607,12 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
         for (int k = 0; k < NC; ++k)
 #pragma unroll
           for (int i = 0; i < OD; ++i)
-            o[k][j][i] = fmaf(c[k][i / 2][i % 2 * 2] + c[k][i / 2][i % 2 * 2 + 1], un, o[k][j][i]);
+            o[k][j][i] += c[k][i / 2][i % 2 * 2] + c[k][i / 2][i % 2 * 2 + 1];
       }
 
       // the stage is read: fetch the tile NST ahead into it
       __syncwarp();
-      if (T + C::NST < w1) {
-        if (lane == 0) load(nxt, st);
-        advance(nxt);
-      }
+      if (T + C::NST < w1) fetch(st);
       if (++st == C::NST) st = 0, phase ^= 1;
 
       const Cursor was = cur;
@@ -598,53 +642,54 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
   __syncthreads();
 
   // Partial results of neighbouring warps with the same head group meet: runs
-  // of slots in warp order.  A run that is the whole head group is written
-  // out, another goes to the CTA's workspace slot (0: it holds the CTA's first
-  // tile, else 1).
-  int run = -1;
-  for (int i = 0, prev = -1; i < 2 * kWarps; ++i) {
-    const int seg = slot_seg[i];
-    if (seg < 0) continue;
-    const int id = seg & 0x3fffffff;
-    const bool head = id != prev;
-    prev = id;
-    if (head) ++run;
-    if (!head || run % kWarps != warp) continue;
-    // this warp joins the run that starts at slot i
-    auto slot = [&](int s) {
-      const bool last = (s & 1) || (slot_seg[s] & 0x40000000);
-      return last ? reinterpret_cast<const float*>(ring + (s >> 1) * C::NST * C::STAGE)
-                  : reinterpret_cast<const float*>(ring + kWarps * C::NST * C::STAGE) +
-                        (s >> 1) * C::SLOT;
-    };
-    int end = i;
-    for (int s = i; s < 2 * kWarps; ++s) {
-      if (slot_seg[s] < 0) continue;
-      if ((slot_seg[s] & 0x3fffffff) != id) break;
-      end = s;
+  // of slots in warp order, a warp for each of a run's heads.  A run that is
+  // the whole head group is written out, another goes to the CTA's workspace
+  // slot (0: it holds the CTA's first tile, else 1).
+  constexpr unsigned kAll = 0xffffffffu, kInLast = 0x40000000u;
+  const int sg = lane < 2 * kWarps ? slot_seg[lane] : -1;
+  const int id = sg < 0 ? -1 : sg & ~int(kInLast);
+  const unsigned used = __ballot_sync(kAll, sg >= 0);
+  const unsigned below = used & ((1u << lane) - 1);
+  const int before = __shfl_sync(kAll, id, below ? 31 - __clz(below) : lane);
+  unsigned heads_of_runs = __ballot_sync(kAll, sg >= 0 && (!below || before != id));
+  const unsigned in_last = __ballot_sync(kAll, (lane & 1) || (sg & int(kInLast)));
+  auto slot = [&](int s) {
+    return reinterpret_cast<const float*>(
+        (in_last >> s & 1) ? ring + (s >> 1) * C::NST * C::STAGE
+                           : ring + kWarps * C::NST * C::STAGE + (s >> 1) * C::SLOT * 4);
+  };
+  while (heads_of_runs) {
+    const int i = __ffs(heads_of_runs) - 1;
+    heads_of_runs &= heads_of_runs - 1;
+    const unsigned upto = heads_of_runs ? (1u << (__ffs(heads_of_runs) - 1)) - 1 : kAll;
+    const unsigned run = used & upto & ~((1u << i) - 1);
+    const int seg = __shfl_sync(kAll, id, i), m = seg / VH, vh = seg - m * VH;
+    int s0 = 0, nt = c1;
+    if (pl.split) {
+      nt = pre[m + 1] - pre[m];
+      s0 = pre[m] * VH + vh * nt;
     }
-    const int m = id / VH, vh = id % VH, nt = (pre[m + 1] - pre[m]) / VH;
-    const int s0 = pre[m] + vh * nt;
     const bool complete = s0 >= c0 && s0 + nt <= c1;
-    const int per = a.nq / a.kv.nkv, h0 = vh % pl.ngrp * pl.gh, heads = min(pl.gh, per - h0);
-    float* out = a.out + int64_t(m) * a.out_ld + int64_t(vh / pl.ngrp * per + h0) * D;
+    float* out = a.out + int64_t(m) * a.out_ld + int64_t(first_head(vh)) * D;
     float* part = pl.part + (int64_t(blockIdx.x) * 2 + (s0 <= c0 ? 0 : 1)) * C::SLOT;
-    for (int h = 0; h < heads; ++h) {
-      float r = -INFINITY;
-      for (int s = i; s <= end; ++s)
-        if (slot_seg[s] >= 0) r = fmaxf(r, slot(s)[HB * D + h]);
-      float ls = 0.f, acc[(D + 31) / 32] = {};
-      for (int s = i; s <= end; ++s) {
-        if (slot_seg[s] < 0) continue;
-        const float* p = slot(s);
-        const float f = ex2_approx(p[HB * D + h] - r);
-        ls = fmaf(p[HB * D + HB + h], f, ls);
+    for (int h = warp; h < n_heads(vh); h += kWarps) {
+      // lanes as slots: their reference points and sums
+      const bool on = run >> lane & 1;
+      const float rs = on ? slot(lane)[HB * D + h] : -INFINITY;
+      const float r = warp_max(rs), f = on ? ex2_approx(rs - r) : 0.f;
+      const float ls = warp_sum(on ? f * slot(lane)[HB * D + HB + h] : 0.f);
+      constexpr int Q = (D + 31) / 32;
+      float acc[Q] = {};
+      for (unsigned w = run; w; w &= w - 1) {
+        const int s = __ffs(w) - 1;
+        const float* p = slot(s) + h * D;
+        const float fs = __shfl_sync(kAll, f, s);
 #pragma unroll
-        for (int q = 0; q < (D + 31) / 32; ++q)
-          if (q * 32 + lane < D) acc[q] = fmaf(p[h * D + q * 32 + lane], f, acc[q]);
+        for (int q = 0; q < Q; ++q)
+          if (q * 32 + lane < D) acc[q] = fmaf(p[q * 32 + lane], fs, acc[q]);
       }
 #pragma unroll
-      for (int q = 0; q < (D + 31) / 32; ++q)
+      for (int q = 0; q < Q; ++q)
         if (q * 32 + lane < D) {
           if (complete) out[h * D + q * 32 + lane] = acc[q] / ls;
           else part[h * D + q * 32 + lane] = acc[q];
@@ -655,55 +700,105 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
 }
 
 // The head groups that several CTAs shared, joined from the workspace (one
-// CTA each), and zeros for empty streams.
+// CTA each), and zeros for empty streams.  A thread takes 4 columns of one
+// head of every SL-th partial result, so that their loads are in flight
+// together.
+constexpr int kJoinThreads = 256;
 template <int D, int NC>
-__global__ void __launch_bounds__(D * 4) attn_kv4_join_kernel(const Plan pl, int grid) {
+__global__ void __launch_bounds__(kJoinThreads) attn_kv4_join_kernel(const Plan pl, int grid) {
   using C = Cfg<D, NC>;
-  __shared__ int sums[2][D * 4 / 32];
+  constexpr int HB = C::HB, ITEMS = HB * D / 4;
+  constexpr int SL = ITEMS < kJoinThreads ? kJoinThreads / ITEMS : 1;
+  extern __shared__ float fac[];  // [partial][HB] weights
+  __shared__ int sums[2][kJoinThreads / 32];
+  __shared__ float lsum[HB];
+  __shared__ float4 acc_s[SL > 1 ? kJoinThreads : 1];
   const AttnKv4Args& a = pl.a;
-  const int VH = pl.VH, m = blockIdx.x / VH, vh = blockIdx.x % VH, tid = threadIdx.x;
+  const int VH = pl.VH, m = blockIdx.x / VH, vh = blockIdx.x - m * VH, tid = threadIdx.x;
+  const int warp = tid >> 5, lane = tid & 31;
   pdl_trigger();
   pdl_wait();
+  auto tiles = [&](int i) { return (clamped_len(a, i) + C::TK - 1) / C::TK; };
   int before = 0, total = 0;
-  for (int i = tid; i < a.kv.M; i += blockDim.x) {
-    const int n = (clamped_len(a, i) + C::TK - 1) / C::TK * VH;
+  for (int i = tid; i < a.kv.M; i += kJoinThreads) {
+    const int n = tiles(i);
     total += n;
     if (i < m) before += n;
   }
   before = __reduce_add_sync(0xffffffffu, before);
   total = __reduce_add_sync(0xffffffffu, total);
-  if (tid % 32 == 0) sums[0][tid / 32] = before, sums[1][tid / 32] = total;
+  if (lane == 0) sums[0][warp] = before, sums[1][warp] = total;
+  const int nt = tiles(m);
   __syncthreads();
   before = total = 0;
-  for (int w = 0; w < D * 4 / 32; ++w) before += sums[0][w], total += sums[1][w];
-  const int nt = (clamped_len(a, m) + C::TK - 1) / C::TK;
-  const int per = a.nq / a.kv.nkv, h0 = vh % pl.ngrp * pl.gh, heads = min(pl.gh, per - h0);
-  float* out = a.out + int64_t(m) * a.out_ld + int64_t(vh / pl.ngrp * per + h0) * D;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) before += sums[0][w], total += sums[1][w];
+  const int per = a.nq / a.kv.nkv, g0 = (vh & ((1 << pl.gsh) - 1)) * pl.gh;
+  const int heads = min(pl.gh, per - g0);
+  float* out = a.out + int64_t(m) * a.out_ld + int64_t((vh >> pl.gsh) * per + g0) * D;
   if (nt == 0) {
-    for (int i = tid; i < heads * D; i += blockDim.x) out[i] = 0.f;
+    for (int i = tid; i < heads * D; i += kJoinThreads) out[i] = 0.f;
     return;
   }
-  const int s0 = before + vh * nt, s1 = s0 + nt;
+  total *= VH;
+  const int s0 = before * VH + vh * nt, s1 = s0 + nt;
   grid = min(grid, total);  // every CTA that has a run has a tile
   // the CTA whose run holds tile T
   auto owner = [&](int T) { return int((int64_t(T + 1) * grid - 1) / total); };
-  const int b0 = owner(s0), b1 = owner(s1 - 1);
-  if (b0 == b1) return;
-  auto slot = [&](int b) {
-    return pl.part + (int64_t(b) * 2 + (s0 <= first_tile(b, grid, total) ? 0 : 1)) * C::SLOT;
+  const int b0 = owner(s0), nb = owner(s1 - 1) - b0 + 1;
+  if (nb == 1) return;
+  // only the first of the CTAs can have begun before this head group
+  const int first = s0 <= first_tile(b0, grid, total) ? 0 : 1;
+  auto slot = [&](int i) {
+    return pl.part + (int64_t(b0 + i) * 2 + (i == 0 ? first : 0)) * C::SLOT;
   };
-  for (int i = tid; i < heads * D; i += blockDim.x) {
-    const int h = i / D;
-    float r = -INFINITY;
-    for (int b = b0; b <= b1; ++b) r = fmaxf(r, __ldcg(slot(b) + C::HB * D + h));
-    float ls = 0.f, acc = 0.f;
-    for (int b = b0; b <= b1; ++b) {
-      const float* p = slot(b);
-      const float f = ex2_approx(__ldcg(p + C::HB * D + h) - r);
-      ls = fmaf(__ldcg(p + C::HB * D + C::HB + h), f, ls);
-      acc = fmaf(__ldcg(p + i), f, acc);
+  for (int h = warp; h < heads; h += kJoinThreads / 32) {
+    float r = -INFINITY, ls = 0.f;
+    for (int i = lane; i < nb; i += 32) {
+      const float v = __ldcg(slot(i) + HB * D + h);
+      fac[i * HB + h] = v;
+      r = fmaxf(r, v);
     }
-    out[i] = acc / ls;
+    r = warp_max(r);
+    for (int i = lane; i < nb; i += 32) {
+      const float f = ex2_approx(fac[i * HB + h] - r);
+      fac[i * HB + h] = f;
+      ls = fmaf(__ldcg(slot(i) + HB * D + HB + h), f, ls);
+    }
+    ls = warp_sum(ls);
+    if (lane == 0) lsum[h] = ls;
+  }
+  __syncthreads();
+  for (int it = tid % ITEMS; it < heads * (D / 4); it += kJoinThreads) {
+    const int h = it / (D / 4);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = SL > 1 ? tid / ITEMS : 0; i < nb; i += SL) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(i)) + it);
+      const float f = fac[i * HB + h];
+      acc.x = fmaf(v.x, f, acc.x);
+      acc.y = fmaf(v.y, f, acc.y);
+      acc.z = fmaf(v.z, f, acc.z);
+      acc.w = fmaf(v.w, f, acc.w);
+    }
+    if constexpr (SL > 1) acc_s[tid] = acc;
+    else {
+      const float f = 1.0f / lsum[h];
+      reinterpret_cast<float4*>(out)[it] = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+    }
+  }
+  if constexpr (SL > 1) {
+    __syncthreads();
+    if (tid < heads * (D / 4)) {
+      float4 acc = acc_s[tid];
+#pragma unroll
+      for (int s = 1; s < SL; ++s) {
+        const float4 v = acc_s[s * ITEMS + tid];
+        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+      }
+      const float f = 1.0f / lsum[tid / (D / 4)];
+      reinterpret_cast<float4*>(out)[tid] = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+    }
   }
 }
 
@@ -750,7 +845,8 @@ cudaError_t launch(K kern, int grid, int threads, int smem, cudaStream_t s, bool
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-// Query heads a head group: at most 8 (two column tiles).
+// Head groups of a kv head: one or two of at most 8 query heads (two column
+// tiles).
 int head_groups(int per) { return (per + 7) / 8; }
 
 template <int D, int NC>
@@ -759,9 +855,10 @@ cudaError_t run(const AttnKv4Args& a, cudaStream_t s, bool pdl) {
   Plan pl;
   const int per = a.nq / a.kv.nkv;
   pl.a = a;
-  pl.ngrp = head_groups(per);
-  pl.gh = (per + pl.ngrp - 1) / pl.ngrp;
-  pl.VH = a.kv.nkv * pl.ngrp;
+  const int groups_kv = head_groups(per);
+  pl.gsh = groups_kv - 1;
+  pl.gh = (per + groups_kv - 1) / groups_kv;
+  pl.VH = a.kv.nkv * groups_kv;
   pl.part = static_cast<float*>(a.ws);
   CUtensorMap km = {}, vm = {};
   if (C::MAP && (!code_map(&km, a.kv.kc, a.kv, C::TK) || !code_map(&vm, a.kv.vc, a.kv, C::TK)))
@@ -771,7 +868,8 @@ cudaError_t run(const AttnKv4Args& a, cudaStream_t s, bool pdl) {
   const int grid = pl.split ? a.num_sms * C::CTAS : int(groups);
   TMG_CUDA_TRY(launch(attn_kv4_kernel<D, NC>, grid, kWarps * 32, C::SMEM, s, pdl, km, vm, pl));
   if (!pl.split) return cudaSuccess;
-  return launch(attn_kv4_join_kernel<D, NC>, int(groups), D * 4, 0, s, true, pl, grid);
+  return launch(attn_kv4_join_kernel<D, NC>, int(groups), kJoinThreads, grid * C::HB * 4, s, true,
+                pl, grid);
 }
 
 template <int D, int NC>
