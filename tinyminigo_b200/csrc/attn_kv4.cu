@@ -30,7 +30,6 @@ namespace tmg {
 
 namespace {
 
-constexpr int kWarps = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // A warp's tile is TK positions of one head: 64, and 32 for head dim 128, so
@@ -41,11 +40,13 @@ struct Cfg {
   static constexpr int G = D < 32 ? D : 32, NG = D / G, TK = D == 128 ? 32 : 64;
   static constexpr int HB = 4 * NC;
   static constexpr int CODE = TK * D / 2, PAR = TK * NG * 4, STAGE = 2 * (CODE + PAR);
+  // One CTA an SM: of two, the one that started first runs ahead of the other
+  // (65 and 82 us of the same work), of one's warps none does.
+  static constexpr int W = NC == 1 ? 16 : 8;        // warps (128 and 255 registers a thread)
   static constexpr int NST = NC == 1 ? 2 : 4;       // stages of a warp's ring
-  static constexpr int CTAS = NC == 1 ? 2 : 1;      // CTAs an SM
   static constexpr int SLOT = HB * (D + 2);         // floats of a partial result (a multiple of 4)
-  static constexpr bool MAP = D >= 64;              // tiles by tensor map (swizzled)
-  static constexpr int SMEM = kWarps * (NST * STAGE + SLOT * 4) + 512;
+  static constexpr bool MAP = D >= 128;              // tiles by tensor map (swizzled)
+  static constexpr int SMEM = W * (NST * STAGE + SLOT * 4) + 1024;
 };
 
 // 2^x by the SFU's ex2 instruction (relative error about 2^-22; 2^-inf = 0)
@@ -98,6 +99,19 @@ __device__ __forceinline__ uint32_t centred_hi(uint32_t x) {
       : "r"(and_or(x, 0x00f000f0u, 0x64006400u)), "r"(0x2c002c00u), "r"(0xd480d480u));
   return y;  // / 16 - 72
 }
+// Four 8x8 matrices of 16-bit elements, rows of 16 bytes: lane i gives the
+// address of row i % 8 of matrix i / 8, and receives of each matrix word t of
+// row g (lane = 4 g + t), or, transposed, element g of rows 2 t and 2 t + 1.
+__device__ __forceinline__ void ldsm(uint32_t a, uint32_t (&w)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+               : "r"(a));
+}
+__device__ __forceinline__ void ldsm_t(uint32_t a, uint32_t (&w)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+               : "r"(a));
+}
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
@@ -114,31 +128,29 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[N]) {
   else
     w[0] = lds32(a);
 }
-__device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint64_t* bar, int row,
+__device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint64_t* bar, int line,
                                          int seg) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(seg)
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(line), "r"(seg)
       : "memory");
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
-// Byte offset in a tile of 16-byte chunk `c` of row `r` as the tensor map's
-// swizzle lays it out (64-byte rows: chunk ^ (r / 2) % 4; 32-byte rows: chunk
-// ^ (r / 4) % 2), so that 8 rows' words of one chunk lie in 32 banks.
+// Byte offset in a tile of 16-byte chunk `c` of row `r`.  Rows of 64 and 32
+// bytes lie in 128-byte lines as the tensor map's swizzle writes them (chunk
+// ^ line % 8 of the line's 8 chunks), so that the words of one chunk of 8
+// rows lie in 32 banks.
 template <int D>
 __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
-  if constexpr (D == 128) return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
-  if constexpr (D == 64) return r * 32 + ((c ^ ((r >> 2) & 1)) << 4);
-  return r * (D / 2);
+  if constexpr (D >= 128) {
+    constexpr int R = 256 / D;  // rows a line
+    return (r / R) * 128 + ((((r % R) * (D / 32) + c) ^ (r / R % 8)) << 4);
+  }
+  return r * (D / 2) + c * 16;
 }
-// Row r of a 16-row matrix operand is position key_of(r) of its 16: the
-// value operand's lane t then reads positions t, t + 4, t + 8, t + 12, whose
-// rows lie in different banks.
-__device__ __forceinline__ int key_of(int r) { return (r & 8) + ((r & 7) >> 1) + 4 * (r & 1); }
-
 // The tiles of all streams, in order of (stream, head group, tile).
 struct Plan {
   AttnKv4Args a;
@@ -161,15 +173,15 @@ struct Cursor {
 };
 
 template <int D, int NC>
-__global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
+__global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
     attn_kv4_kernel(const __grid_constant__ CUtensorMap kmap,
                     const __grid_constant__ CUtensorMap vmap, const Plan pl) {
   using C = Cfg<D, NC>;
-  constexpr int G = C::G, NG = C::NG, TK = C::TK, KB = TK / 16, HB = C::HB;
+  constexpr int G = C::G, NG = C::NG, TK = C::TK, KB = TK / 16, HB = C::HB, kWarps = C::W;
   constexpr int OD = D == 16 ? 2 : 4;  // output dims a lane and group
   extern __shared__ uint8_t smem[];
-  // 512: the period of the widest swizzle
-  uint8_t* ring = smem + (-smem_u32(smem) & 511u);
+  // 1024: the period of the swizzle (a stage is a multiple of it)
+  uint8_t* ring = smem + (-smem_u32(smem) & 1023u);
   __shared__ __align__(8) uint64_t full[kWarps][C::NST];
   __shared__ int pre[kKv4MaxStreams + 1];  // tiles before each stream
   __shared__ int scan_s[kWarps];
@@ -289,8 +301,8 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
     const uint32_t pb = n * NG * 4;
     if constexpr (C::MAP) {
       mbar_expect_tx(bar, 2 * (C::CODE + pb));
-      tma_tile(s, &kmap, bar, row, seg);
-      tma_tile(s + C::CODE, &vmap, bar, row, seg);
+      tma_tile(s, &kmap, bar, row / (256 / D), seg);
+      tma_tile(s + C::CODE, &vmap, bar, row / (256 / D), seg);
     } else {
       const uint32_t cb = n * (D / 2);
       mbar_expect_tx(bar, 2 * (cb + pb));
@@ -310,23 +322,34 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
   // dims 4 g .. (2 g .. for head dim 16) of each group
   float ref[NC], l[NC], cm[NC][NG], o[NC][NG][OD], cq[NC], qs[NC][NG];
   uint32_t qb[NC][NG][4];
-  auto start = [&](const Cursor& c) {
+  // as an operand the lane holds head g / 2 (part g % 2), of each group the
+  // elements that lane t's code words hold
+  constexpr int E = D == 16 ? 4 : 8;
+  auto load_q = [&](const Cursor& c, float4 (&v)[NC][NG][E / 4]) {
     const int heads = n_heads(c.vh);
     const float* q = a.q + int64_t(c.m) * a.q_ld + int64_t(first_head(c.vh)) * D;
 #pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i) {
+          const int h = 4 * k + g / 2;
+          v[k][j][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (h < heads)
+            v[k][j][i] = *reinterpret_cast<const float4*>(q + h * D + j * G + t * E + 4 * i);
+        }
+  };
+  auto start = [&](const float4 (&q)[NC][NG][E / 4]) {
+#pragma unroll
     for (int k = 0; k < NC; ++k) {
-      // as an operand the lane holds head g / 2 (part g % 2), of each group
-      // the elements that lane t's code words hold
-      const int h = 4 * k + g / 2;
-      constexpr int E = D == 16 ? 4 : 8;
       float x[NG][E];
       float big = 0.f;
 #pragma unroll
       for (int j = 0; j < NG; ++j)
 #pragma unroll
         for (int i = 0; i < E; i += 4) {
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (h < heads) v = *reinterpret_cast<const float4*>(q + h * D + j * G + t * E + i);
+          const float4 v = q[k][j][i / 4];
           x[j][i] = v.x, x[j][i + 1] = v.y, x[j][i + 2] = v.z, x[j][i + 3] = v.w;
           big = fmaxf(big, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
         }
@@ -432,12 +455,17 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
         nxt_head = head_of(nxt);
       }
     };
+    float4 q[NC][NG][E / 4];
+    load_q(cur, q);
+    int len = clamped_len(a, cur.m);
     for (int i = 0; i < C::NST && w0 + i < w1; ++i) fetch(i);
     const int seg_first = cur.m * VH + cur.vh;
-    start(cur);
-    int len = clamped_len(a, cur.m);
+    start(q);
     bool whole = cur.tile == 0;  // the head group began in this warp
-    const int kg = key_of(g);
+    // the row that this lane addresses in a ldmatrix of 16 positions and two
+    // groups (D >= 64; of 32 positions for D = 32): matrices in order (8 rows,
+    // next 8 rows) x groups
+    const int lrow = D == 32 ? lane : lane & 15, lgrp = D == 32 ? 0 : lane >> 4;
     int st = 0;
     uint32_t phase = 0;
     for (int T = w0; T < w1; ++T) {
@@ -449,28 +477,35 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
       const uint32_t base = smem_u32(my_ring + st * C::STAGE);
       const int valid = len - cur.tile * TK;  // positions of the tile in the row
 
-      // scores of positions 16 b + 8 i + kg, x[][2 b + i]
+      // scores of positions 16 b + 8 i + g, x[][2 b + i]
+      [[maybe_unused]] uint32_t kw[4];
       float x[NC][2 * KB];
 #pragma unroll
       for (int b = 0; b < KB; ++b) {
-        uint32_t p0[NG], p1[NG];
-        lds_words<NG>(base + 2 * C::CODE + (16 * b + kg) * NG * 4, p0);
-        lds_words<NG>(base + 2 * C::CODE + (16 * b + 8 + kg) * NG * 4, p1);
+        uint32_t p0[NG], p1[NG], w[NG][2];  // parameters and code words of the two rows
+        lds_words<NG>(base + 2 * C::CODE + (16 * b + g) * NG * 4, p0);
+        lds_words<NG>(base + 2 * C::CODE + (16 * b + 8 + g) * NG * 4, p1);
+        if constexpr (D == 16) {  // two bytes: one to each half
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            w[0][i] = __byte_perm(lds32(base + (16 * b + 8 * i + g) * 8 + (t >> 1) * 4), 0u,
+                                  t & 1 ? 0x4342u : 0x4140u);
+        } else if constexpr (D == 32) {
+          if (b % 2 == 0) ldsm(base + (16 * b + lrow) * 16, kw);
+          w[0][0] = kw[b % 2 * 2], w[0][1] = kw[b % 2 * 2 + 1];
+        } else {
+#pragma unroll
+          for (int j = 0; j < NG; j += 2) {
+            uint32_t v[4];
+            ldsm(base + chunk_off<D>(16 * b + lrow, j + lgrp), v);
+            w[j][0] = v[0], w[j][1] = v[1], w[j + 1][0] = v[2], w[j + 1][1] = v[3];
+          }
+        }
 #pragma unroll
         for (int k = 0; k < NC; ++k) x[k][2 * b] = x[k][2 * b + 1] = 0.f;
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-          uint32_t u, v;
-          if constexpr (D == 16) {  // two bytes: one to each half
-            u = lds32(base + chunk_off<D>(16 * b + kg, 0) + (t >> 1) * 4);
-            v = lds32(base + chunk_off<D>(16 * b + 8 + kg, 0) + (t >> 1) * 4);
-            const uint32_t sel = t & 1 ? 0x4342u : 0x4140u;
-            u = __byte_perm(u, 0u, sel);
-            v = __byte_perm(v, 0u, sel);
-          } else {
-            u = lds32(base + chunk_off<D>(16 * b + kg, j) + t * 4);
-            v = lds32(base + chunk_off<D>(16 * b + 8 + kg, j) + t * 4);
-          }
+          const uint32_t u = w[j][0], v = w[j][1];
           const float s0 = kv4_step(p0[j]), m0 = kv4_min(p0[j]);
           const float s1 = kv4_step(p1[j]), m1 = kv4_min(p1[j]);
 #pragma unroll
@@ -490,11 +525,11 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
       uint32_t pv[2 * KB][NG];  // the values' parameters of the same positions
 #pragma unroll
       for (int i = 0; i < 2 * KB; ++i)
-        lds_words<NG>(base + 2 * C::CODE + C::PAR + (8 * i + kg) * NG * 4, pv[i]);
+        lds_words<NG>(base + 2 * C::CODE + C::PAR + (8 * i + g) * NG * 4, pv[i]);
       if (valid < TK) {
 #pragma unroll
         for (int i = 0; i < 2 * KB; ++i)
-          if (8 * i + kg >= valid) {  // whatever the rows behind the last hold
+          if (8 * i + g >= valid) {  // whatever the rows behind the last hold
 #pragma unroll
             for (int k = 0; k < NC; ++k) x[k][i] = -INFINITY;
 #pragma unroll
@@ -559,6 +594,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
           p[k][i] = ex2_approx(fmaf(x[k][i], cq[k], -ref[k]));
           l[k] += p[k][i];
         }
+      [[maybe_unused]] uint32_t vw[KB][4];
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         uint32_t pb[NC][2 * KB];
@@ -574,33 +610,35 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
         float c[NC][2][4] = {};
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
-          // the codes of the lane's dims of positions t, t + 4 | t + 8, t + 12
-          uint32_t w[4];
+          // the codes of 4 dims of positions 16 b + 2 t, + 1 (u) and + 8, + 9 (v)
+          uint32_t u, v;
+          if constexpr (D == 16) {  // byte g of the rows
+            uint32_t w[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 16 * b + 4 * i + t;
-            w[i] = lds32(base + C::CODE + chunk_off<D>(r, j) + (D == 16 ? g >> 2 : g >> 1) * 4);
-          }
-          if constexpr (D == 16) {
-            const uint32_t sel = (g & 3) * 0x0101u + 0x0400u;  // byte g of both
-            const uint32_t u = __byte_perm(w[0], w[1], (sel & 0xfu) | ((sel >> 8 & 0xfu) << 8));
-            const uint32_t v = __byte_perm(w[2], w[3], (sel & 0xfu) | ((sel >> 8 & 0xfu) << 8));
-#pragma unroll
-            for (int k = 0; k < NC; ++k)
-              mma_f16(c[k][0], centred_lo(u), centred_hi(u), centred_lo(v), centred_hi(v),
-                      pb[k][2 * b], pb[k][2 * b + 1]);
+            for (int i = 0; i < 4; ++i)
+              w[i] = lds32(base + C::CODE + (16 * b + 8 * (i >> 1) + 2 * t + (i & 1)) * 8 +
+                           (g >> 2) * 4);
+            const uint32_t sel = (g & 3) | (4 + (g & 3)) << 8;
+            u = __byte_perm(w[0], w[1], sel);
+            v = __byte_perm(w[2], w[3], sel);
+          } else if constexpr (D == 32) {
+            if (b % 2 == 0) ldsm_t(base + C::CODE + (16 * b + lrow) * 16, vw[0]);
+            u = vw[0][b % 2 * 2], v = vw[0][b % 2 * 2 + 1];
           } else {
-            const uint32_t sel = g & 1 ? 0x7632u : 0x5410u;
-            const uint32_t u = __byte_perm(w[0], w[1], sel), v = __byte_perm(w[2], w[3], sel);
-            const uint32_t a0 = centred_lo(u), a1 = centred_hi(u);
-            const uint32_t a2 = centred_lo(v), a3 = centred_hi(v);
+            if (j % 2 == 0) ldsm_t(base + C::CODE + chunk_off<D>(16 * b + lrow, j + lgrp), vw[b]);
+            u = vw[b][j % 2 * 2], v = vw[b][j % 2 * 2 + 1];
+          }
+          const uint32_t a0 = centred_lo(u), a1 = centred_hi(u);
+          const uint32_t a2 = centred_lo(v), a3 = centred_hi(v);
+#pragma unroll
+          for (int k = 0; k < NC; ++k)
+            mma_f16(c[k][0], a0, a1, a2, a3, pb[k][2 * b], pb[k][2 * b + 1]);
+          if constexpr (D > 16) {
             const uint32_t b0 = centred_lo(u >> 8), b1 = centred_hi(u >> 8);
             const uint32_t b2 = centred_lo(v >> 8), b3 = centred_hi(v >> 8);
 #pragma unroll
-            for (int k = 0; k < NC; ++k) {
-              mma_f16(c[k][0], a0, a1, a2, a3, pb[k][2 * b], pb[k][2 * b + 1]);
+            for (int k = 0; k < NC; ++k)
               mma_f16(c[k][1], b0, b1, b2, b3, pb[k][2 * b], pb[k][2 * b + 1]);
-            }
           }
         }
 #pragma unroll
@@ -630,8 +668,9 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<D, NC>::CTAS)
           if (lane == 0 && first && T + 1 == w1) slot_seg[2 * warp] = seg | 0x40000000;
         }
         if (T + 1 < w1) {
-          start(cur);
+          load_q(cur, q);
           len = clamped_len(a, cur.m);
+          start(q);
           whole = true;
         }
       }
@@ -815,18 +854,19 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
   return fn;
 }
 
-// A map over the codes [M * nkv, cap, d / 2] with a box of `rows` rows; a
-// box reaching behind a head's last row reads zeros there.
+// A map over the codes as 128-byte lines (2 or 4 rows) of each head [M * nkv,
+// cap * d / 256, 128] with a box of `rows` rows: TMA moves a line a step, and
+// 64 steps for rows of 32 bytes took 4 us to fill the rings.  A box reaching
+// behind a head's last line reads zeros there.
 bool code_map(CUtensorMap* map, const uint8_t* base, const Kv4& kv, int rows) {
   auto fn = encode_tiled();
   if (!fn) return false;
-  const cuuint64_t row = kv.d / 2;
-  const cuuint64_t dims[3] = {row, cuuint64_t(kv.cap), cuuint64_t(kv.M) * kv.nkv};
-  const cuuint64_t strides[2] = {row, row * kv.cap};
-  const cuuint32_t box[3] = {cuuint32_t(row), cuuint32_t(rows), 1}, estr[3] = {1, 1, 1};
+  const cuuint64_t lines = cuuint64_t(kv.cap) * kv.d / 256;  // cap % 4 == 0
+  const cuuint64_t dims[3] = {128, lines, cuuint64_t(kv.M) * kv.nkv};
+  const cuuint64_t strides[2] = {128, lines * 128};
+  const cuuint32_t box[3] = {128, cuuint32_t(rows * kv.d / 256), 1}, estr[3] = {1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(base), dims, strides, box,
-            estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            kv.d == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -865,8 +905,8 @@ cudaError_t run(const AttnKv4Args& a, cudaStream_t s, bool pdl) {
     return cudaErrorInvalidValue;
   const int64_t groups = int64_t(a.kv.M) * pl.VH;
   pl.split = a.max_len > 16 * C::TK;
-  const int grid = pl.split ? a.num_sms * C::CTAS : int(groups);
-  TMG_CUDA_TRY(launch(attn_kv4_kernel<D, NC>, grid, kWarps * 32, C::SMEM, s, pdl, km, vm, pl));
+  const int grid = pl.split ? a.num_sms : int(groups);
+  TMG_CUDA_TRY(launch(attn_kv4_kernel<D, NC>, grid, C::W * 32, C::SMEM, s, pdl, km, vm, pl));
   if (!pl.split) return cudaSuccess;
   return launch(attn_kv4_join_kernel<D, NC>, int(groups), kJoinThreads, grid * C::HB * 4, s, true,
                 pl, grid);
@@ -898,8 +938,7 @@ cudaError_t attn_kv4_prepare() {
 
 size_t attn_kv4_ws(const Kv4& kv, int nq, int num_sms) {
   const int nc = column_tiles(nq / kv.nkv);
-  // Cfg's CTAS and SLOT
-  return size_t(num_sms) * (nc == 1 ? 2 : 1) * 2 * (4 * nc) * (kv.d + 2) * 4;
+  return size_t(num_sms) * 2 * (4 * nc) * (kv.d + 2) * 4;  // two of Cfg's SLOT a CTA
 }
 
 cudaError_t launch_attn_kv4(const AttnKv4Args& a, cudaStream_t s, bool pdl) {
