@@ -209,30 +209,44 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
   // this CTA's tiles [c0, c1)
   int c0, c1;
   if (pl.split) {
-    // tiles (of one head group) before each stream: 4 streams a thread,
-    // scanned over the CTA
-    int n[4], sum = 0;
+    // tiles (of one head group) before each stream: by the first warp, or 4
+    // streams a thread, scanned over the CTA
+    if (M <= 32) {
+      if (warp == 0) {
+        const int n = lane < M ? checked_tiles(lane) : 0;
+        int inc = n;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      n[i] = 4 * tid + i < M ? checked_tiles(4 * tid + i) : 0;
-      sum += n[i];
-    }
-    int inc = sum;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += v;
+        }
+        if (lane <= M) pre[lane] = inc - n;
+        if (M == 32 && lane == 31) pre[32] = inc;
+      }
+    } else {
+      int n[4], sum = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    if (lane == 31) scan_s[warp] = inc;
-    __syncthreads();
-    int at = inc - sum;
-    for (int w = 0; w < warp; ++w) at += scan_s[w];
+      for (int i = 0; i < 4; ++i) {
+        n[i] = 4 * tid + i < M ? checked_tiles(4 * tid + i) : 0;
+        sum += n[i];
+      }
+      int inc = sum;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (4 * tid + i <= M) pre[4 * tid + i] = at;
-      at += n[i];
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (lane == 31) scan_s[warp] = inc;
+      __syncthreads();
+      int at = inc - sum;
+      for (int w = 0; w < warp; ++w) at += scan_s[w];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (4 * tid + i <= M) pre[4 * tid + i] = at;
+        at += n[i];
+      }
+      if (M == kKv4MaxStreams && tid == kWarps * 32 - 1) pre[M] = at;
     }
-    if (M == kKv4MaxStreams && tid == kWarps * 32 - 1) pre[M] = at;
     __syncthreads();
     const int total = pre[M] * VH, ctas = min(int(gridDim.x), total);
     if (int(blockIdx.x) >= ctas) return;
@@ -719,13 +733,17 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
       const float ls = warp_sum(on ? f * slot(lane)[HB * D + HB + h] : 0.f);
       constexpr int Q = (D + 31) / 32;
       float acc[Q] = {};
-      for (unsigned w = run; w; w &= w - 1) {
-        const int s = __ffs(w) - 1;
-        const float* p = slot(s) + h * D;
+      // each warp from the run's first to its last has one of its slots, or none
+      const int wb = (31 - __clz(run)) >> 1;
+#pragma unroll 4
+      for (int w = i >> 1; w <= wb; ++w) {
+        const unsigned which = run >> (2 * w) & 3;
+        const int s = 2 * w + (which >> 1);
         const float fs = __shfl_sync(kAll, f, s);
+        const float* p = slot(s) + h * D;
 #pragma unroll
         for (int q = 0; q < Q; ++q)
-          if (q * 32 + lane < D) acc[q] = fmaf(p[q * 32 + lane], fs, acc[q]);
+          if (which && q * 32 + lane < D) acc[q] = fmaf(p[q * 32 + lane], fs, acc[q]);
       }
 #pragma unroll
       for (int q = 0; q < Q; ++q)
