@@ -2831,7 +2831,7 @@ int tmg_op_logprobs(tmg_ctx* c, const float* logits, int64_t ld, int64_t rows, i
   a.top_ids = top_ids;
   a.top_logprobs = top_logprobs;
   a.err = c->d_err;
-  CK(launch_logprobs(a, c->stream), "logprobs");
+  CK(launch_logprobs(a, c->stream, c->num_sms), "logprobs");
   return TMG_OK;
 }
 

@@ -369,7 +369,7 @@ struct LogprobsArgs {
   float* top_logprobs = nullptr;  // [rows, n_top]
   int32_t* err = nullptr;
 };
-cudaError_t launch_logprobs(const LogprobsArgs& a, cudaStream_t s);
+cudaError_t launch_logprobs(const LogprobsArgs& a, cudaStream_t s, int num_sms);
 int sample_slices(int64_t V, int M, int num_sms);
 
 }  // namespace tmg
