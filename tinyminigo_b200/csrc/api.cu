@@ -2807,7 +2807,7 @@ int tmg_op_attn_decode_kv4(tmg_ctx* c, const tmg_kv4* view, const float* q, int6
 int tmg_op_logprobs(tmg_ctx* c, const float* logits, int64_t ld, int64_t rows, int64_t V,
                     const uint32_t* targets, int32_t n_top, float* logprob, float* entropy,
                     uint32_t* top_ids, float* top_logprobs) {
-  if (!c || !logits || V <= 0 || V > INT32_MAX || ld < V || rows < 0 || rows > INT32_MAX)
+  if (!c || !logits || V <= 0 || V > (1 << 30) || ld < V || rows < 0 || rows > INT32_MAX)
     return fail(c, TMG_ERR_INVALID, "tmg_op_logprobs: bad argument");
   if ((reinterpret_cast<uintptr_t>(logits) & 3) != 0)
     return fail(c, TMG_ERR_INVALID, "tmg_op_logprobs: logits must be 4-byte aligned");

@@ -19,7 +19,9 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kCand = 2048;  // candidates of a row held in shared memory
+constexpr int kCand = 2048;  // candidates of a slice held in shared memory
+constexpr int kSlack = 2;    // threads more than wanted that a bound may let through
+constexpr int kMaxSlices = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 using u64 = unsigned long long;
@@ -59,68 +61,46 @@ __device__ __forceinline__ void move(Soft& s, float x) {
   s.l *= f;
   s.x = x;
 }
-__device__ __forceinline__ void merge(Soft& a, Soft b) {
-  const float x = fmaxf(a.x, b.x);
-  if (x > -INFINITY) {  // else both sums are 0, or NaN
-    move(a, x);
-    move(b, x);
-  }
-  a.l += b.l;
-  a.w += b.w;
-}
-
 // 4 floats of the row at chunk c of the 16-byte grid its first element
 // lies `shift` floats into; elements outside the row read as -inf and
 // have no key.
 struct Row {
   const float* base;  // 16-byte aligned: the row's start - shift
   int shift;
-  int64_t V;
-  __device__ __forceinline__ float4 load(int64_t c) const {
-    const int64_t i = 4 * c - shift;
-    if (i >= 0 && i + 4 <= V) return __ldg(reinterpret_cast<const float4*>(base) + c);
+  int V;
+  __device__ __forceinline__ float4 load(int c) const {
+    const int i = 4 * c - shift;
+    if (i >= 0 && i <= V - 4) return __ldg(reinterpret_cast<const float4*>(base) + c);
     float v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = i + j >= 0 && i + j < V ? __ldg(base + 4 * c + j) : -INFINITY;
+    for (int j = 0; j < 4; ++j) v[j] = i + j >= 0 && i < V - j ? __ldg(base + 4 * int64_t(c) + j) : -INFINITY;
     return make_float4(v[0], v[1], v[2], v[3]);
   }
-  __device__ __forceinline__ u64 key(float x, int64_t c, int j) const {
-    const int64_t i = 4 * c - shift + j;
+  __device__ __forceinline__ u64 key(float x, int c, int j) const {
+    const int i = 4 * c - shift + j;
     return i >= 0 && i < V ? order_key(x, uint32_t(i)) : 0ull;
   }
 };
 
-// The largest of the row's elements in v, as keys; elements outside have none.
-__device__ __forceinline__ u64 best_key(const Row& R, const float4& v, int64_t c) {
-  const float x[4] = {v.x, v.y, v.z, v.w};
-  u64 b = 0ull;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const u64 k = R.key(x[j], c, j);
-    b = k > b ? k : b;
-  }
-  return b;
-}
-
-// A thread's pass over its chunks: the online state, and the first chunk that
-// holds its largest element.
+// A thread's pass over its chunks: the online state, and the index of the
+// first of its largest elements.
 struct Pass {
   Soft s;
-  float best = -INFINITY;
-  int64_t at;
+  uint32_t idx;
   template <int U>
-  __device__ __forceinline__ void take(const float4 (&v)[U], int64_t c) {
-    float m[U], mx = -INFINITY;
+  __device__ __forceinline__ void take(const float4 (&v)[U], int c, int shift) {
+    float mx = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      m[u] = fmaxf(fmaxf(v[u].x, v[u].y), fmaxf(v[u].z, v[u].w));
-      mx = fmaxf(mx, m[u]);
-    }
-    if (mx > best) {
-      best = mx;
+    for (int u = 0; u < U; ++u)
+      mx = fmaxf(mx, fmaxf(fmaxf(v[u].x, v[u].y), fmaxf(v[u].z, v[u].w)));
+    if (mx > s.x) {
 #pragma unroll
-      for (int u = U - 1; u >= 0; --u)
-        if (m[u] == mx) at = c + int64_t(u) * kThreads;
+      for (int u = U - 1; u >= 0; --u) {
+        const float x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+        for (int j = 3; j >= 0; --j)
+          if (x[j] == mx) idx = uint32_t(4 * (c + u * kThreads) + j - shift);
+      }
       move(s, mx);
     }
     const float ref = s.x == -INFINITY ? 0.f : s.x;
@@ -137,125 +117,175 @@ struct Pass {
   }
 };
 
-// The CTA's result, for the cluster's first CTA to join.
-struct Part {
-  Soft s;
-  int n;  // alternatives in the list, largest first
-  u64 top[kMaxTopK];
+// The states of a warp's lanes (of lanes that agree in the bits above `from`)
+// as one: the largest x first, then sums relative to it.
+__device__ __forceinline__ Soft across(Soft s, int from) {
+  float x = s.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o <= from) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  if (x > -INFINITY) move(s, x);  // else the sums are 0, or NaN
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o <= from) {
+      s.l += __shfl_xor_sync(0xffffffffu, s.l, o);
+      s.w += __shfl_xor_sync(0xffffffffu, s.w, o);
+    }
+  return s;
+}
+
+// The slices' results, in the shared memory of the cluster's first CTA.
+struct Parts {
+  float x[kMaxSlices], l[kMaxSlices], w[kMaxSlices];
+  int n[kMaxSlices];  // alternatives in the list, largest first
+  u64 top[kMaxSlices][kMaxTopK];
 };
 
 __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const LogprobsArgs a) {
-  __shared__ Soft soft_s[kThreads / 32];
+  constexpr int kW = kThreads / 32;
+  __shared__ float soft_s[3][kW];
+  __shared__ unsigned or_s[kW], and_s[kW];
   __shared__ u64 cand[kCand];
-  __shared__ int owner[kMaxTopK];
+  __shared__ int owner[kMaxTopK + kSlack];
   __shared__ int n_owner, n_cand, n_s;
-  __shared__ Part part;
+  __shared__ Parts parts;
   cg::cluster_group cluster = cg::this_cluster();
   const int slices = int(cluster.num_blocks()), slice = int(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t r = blockIdx.x / slices;
+  const int64_t r = blockIdx.x / unsigned(slices);
   const float* row = a.logits + r * a.ld;
+  const int V = int(a.V);
   Row R;
   R.shift = int((reinterpret_cast<uintptr_t>(row) >> 2) & 3);
   R.base = row - R.shift;
-  R.V = a.V;
+  R.V = V;
   // this slice's chunks [c0, c1): thread t has c0 + t, c0 + t + kThreads, ..
-  const int64_t nc = (a.V + R.shift + 3) / 4;
-  const int64_t per_slice = (nc + slices - 1) / slices;
-  const int64_t c0 = min(nc, slice * per_slice), c1 = min(nc, c0 + per_slice);
+  const int nc = V / 4 + (V % 4 + R.shift + 3) / 4;
+  const int per_slice = (nc + slices - 1) / slices;
+  const int c0 = min(nc, slice * per_slice), c1 = min(nc, c0 + per_slice);
   if (tid == 0) n_owner = n_cand = 0;
   pdl_trigger();
   pdl_wait();
+  // no CTA writes into the first one's memory before that has started
+  if (slices > 1) cluster.barrier_arrive();
+
+  float at_target = 0.f;  // thread 0: the target's logit, fetched early
+  uint32_t target = 0;
+  if (tid == 0 && slice == 0 && a.logprob) {
+    target = a.targets[r];
+    if (target < uint32_t(V)) at_target = row[target];
+  }
 
   Pass ps;
-  ps.at = c0 + tid;
+  ps.idx = uint32_t(max(4 * (c0 + tid) - R.shift, 0));
   {
     constexpr int U = 4;  // 16-byte loads in flight a thread
-    int64_t c = c0 + tid;
+    int c = c0 + tid;
     // whole chunks only: not the row's first if it is not aligned, nor its last
-    const int64_t whole = min(c1, (a.V + R.shift) / 4);
+    const int whole = min(c1, V / 4 + (V % 4 + R.shift) / 4);
     const float4* p = reinterpret_cast<const float4*>(R.base);
     if (c < c1 && c == 0 && R.shift != 0) {
       const float4 v[1] = {R.load(c)};
-      ps.take(v, c);
+      ps.take(v, c, R.shift);
       c += kThreads;
     }
-    for (; c + (U - 1) * kThreads < whole; c += U * kThreads) {
+    for (; c < whole - (U - 1) * kThreads; c += U * kThreads) {
       float4 v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) v[u] = __ldg(p + c + u * kThreads);
-      ps.take(v, c);
+      ps.take(v, c, R.shift);
     }
+#pragma unroll 1
     for (; c < c1; c += kThreads) {
       const float4 v[1] = {R.load(c)};
-      ps.take(v, c);
+      ps.take(v, c, R.shift);
     }
   }
-  auto across = [&](Soft s, int from) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      if (o > from) continue;
-      Soft u;
-      u.x = __shfl_xor_sync(0xffffffffu, s.x, o);
-      u.l = __shfl_xor_sync(0xffffffffu, s.l, o);
-      u.w = __shfl_xor_sync(0xffffffffu, s.w, o);
-      merge(s, u);
-    }
-    return s;
-  };
+  // for the alternatives, each thread's largest key; and the bits in which
+  // their upper halves differ
+  u64 mine = 0ull;
+  if (a.n_top) {
+    if (c0 + tid < c1) mine = order_key(ps.s.x, ps.idx);
+    const unsigned hi = unsigned(mine >> 32);
+    const unsigned any = __reduce_or_sync(0xffffffffu, hi);
+    const unsigned every = __reduce_and_sync(0xffffffffu, mine ? hi : ~0u);
+    if (lane == 0) or_s[warp] = any, and_s[warp] = every;
+  }
   Soft s = across(ps.s, 16);
-  if (lane == 0) soft_s[warp] = s;
+  if (lane == 0) soft_s[0][warp] = s.x, soft_s[1][warp] = s.l, soft_s[2][warp] = s.w;
   __syncthreads();
-  s = across(soft_s[lane % (kThreads / 32)], kThreads / 64);
+  s.x = soft_s[0][lane % kW], s.l = soft_s[1][lane % kW], s.w = soft_s[2][lane % kW];
+  s = across(s, kW / 2);
 
-  // Alternatives.  Each thread's largest key is an element; the n_top-th
-  // largest of them bounds the slice's n_top-th largest element from below, and
-  // only the n_top threads at or above it can hold an element that is: their
-  // elements are looked at again.
+  // Alternatives.  A thread's largest key is an element; the n_top-th largest of
+  // them (or a bound that a few more reach) bounds the slice's n_top-th largest
+  // element from below, and only the threads at or above it can hold an
+  // element that is: their elements are looked at again.
   int n = 0;
   if (a.n_top) {
-    const u64 mine = ps.at < c1 ? best_key(R, R.load(ps.at), ps.at) : 0ull;
-    u64 tau = 0ull;
-    for (int b = 63; b >= 0; --b) {
-      const u64 t = tau | (1ull << b);
-      const int m = __syncthreads_count(mine >= t);
-      if (m >= a.n_top) tau = t;
-      if (m == a.n_top) break;
+    const unsigned any = __reduce_or_sync(0xffffffffu, or_s[lane % kW]);
+    const unsigned every = __reduce_and_sync(0xffffffffu, and_s[lane % kW]);
+    // the bits above the first in which two keys differ are everybody's
+    int b = 63 - __clz(any ^ every);
+    if (any == every) b = 31;
+    u64 tau = b == 63 ? 0ull : u64(every) << 32 >> (b + 1) << (b + 1);
+    // (a thread without elements, or fewer than n_top threads: tau stays below)
+    if (__syncthreads_count(mine >= tau && mine != 0ull) >= a.n_top) {
+#pragma unroll 1
+      for (; b >= 0; --b) {
+        const u64 t = tau | (1ull << b);
+        const int m = __syncthreads_count(mine >= t);
+        if (m >= a.n_top) tau = t;
+        if (m >= a.n_top && m <= a.n_top + kSlack) break;
+      }
+    } else {
+      tau = 0ull;
     }
-    const int64_t per = (c1 - c0 + kThreads - 1) / kThreads;
-    if (mine >= tau && mine != 0ull) owner[min(atomicAdd(&n_owner, 1), kMaxTopK - 1)] = tid;
+    if (mine >= tau && mine != 0ull) {
+      const int i = atomicAdd(&n_owner, 1);
+      if (i < kMaxTopK + kSlack) owner[i] = tid;
+    }
     __syncthreads();
     const bool all = n_owner < a.n_top;  // fewer threads with elements than wanted
-    const int64_t todo = all ? c1 - c0 : per * n_owner;
+    const int owners = all ? min(kThreads, c1 - c0) : min(n_owner, kMaxTopK + kSlack);
+    const int per = (c1 - c0 + kThreads - 1) / kThreads;
     auto collect = [&](u64 t, bool keep) {
       int m = 0;
-      for (int64_t i = tid; i < todo; i += kThreads) {
-        const int64_t c = c0 + (all ? i : i / n_owner * kThreads + owner[i % n_owner]);
-        if (c >= c1) continue;
-        const float4 v = R.load(c);
-        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll 1
+      for (int w = warp; w < owners; w += kW) {
+        const int first = c0 + (all ? w : owner[w]);
+#pragma unroll 1
+        for (int i = lane; i < per; i += 32) {
+          const int c = first + i * kThreads;
+          if (c >= c1) continue;
+          const float4 v = R.load(c);
+          const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const u64 k = R.key(x[j], c, j);
-          if (k != 0ull && k >= t) {
-            ++m;
-            if (keep) {
-              const int at = atomicAdd(&n_cand, 1);
-              if (at < kCand) cand[at] = k;
+          for (int j = 0; j < 4; ++j) {
+            const u64 k = R.key(x[j], c, j);
+            if (k != 0ull && k >= t) {
+              ++m;
+              if (keep) {
+                const int at = atomicAdd(&n_cand, 1);
+                if (at < kCand) cand[at] = k;
+              }
             }
           }
         }
       }
       return m;
     };
-    collect(tau, true);
-    __syncthreads();
-    if (n_cand > kCand) {
-      // more at or above the bound than fit (few threads hold the large ones):
-      // raise it, bit by bit, to a value that n_top or a few more reach
+    // more at or above the bound than fit (few threads hold the large ones):
+    // raise it, bit by bit, to a value that n_top or a few more reach
+#pragma unroll 1
+    for (int round = 0; round < 2; ++round) {
+      collect(tau, true);
+      __syncthreads();
+      if (n_cand <= kCand) break;
       u64 up = 0ull;
-      for (int b = 63; b >= 0; --b) {
-        const u64 t = up | (1ull << b);
+#pragma unroll 1
+      for (int q = 63; q >= 0; --q) {
+        const u64 t = up | (1ull << q);
         if (tid == 0) n_s = 0;
         __syncthreads();
         const int m = collect(t > tau ? t : tau, false);
@@ -266,67 +296,79 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const LogprobsArg
         if (total >= a.n_top) up = t;
         if (total >= a.n_top && total <= kCand) break;
       }
+      tau = up > tau ? up : tau;
       if (tid == 0) n_cand = 0;
-      __syncthreads();
-      collect(up > tau ? up : tau, true);
       __syncthreads();
     }
     const int m = min(n_cand, kCand);
     n = min(m, a.n_top);
+    if (slices > 1) cluster.barrier_wait();
+    u64* top = slices > 1 ? cluster.map_shared_rank(&parts.top[slice][0], 0) : parts.top[0];
+#pragma unroll 1
     for (int i = tid; i < m; i += kThreads) {
       const u64 k = cand[i];
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < m; ++j) rank += cand[j] > k;
-      if (rank < a.n_top) part.top[rank] = k;
+      if (rank < a.n_top) top[rank] = k;
     }
+  } else if (slices > 1) {
+    cluster.barrier_wait();
   }
-  if (tid == 0) part.s = s, part.n = n;
 
   // The slices meet in the first one's CTA: the states merge, and an
   // alternative's rank is the sum of its ranks in the sorted lists.
   if (slices > 1) {
+    if (tid == 0) {
+      Parts* p = cluster.map_shared_rank(&parts, 0);
+      p->x[slice] = s.x;
+      p->l[slice] = s.l;
+      p->w[slice] = s.w;
+      p->n[slice] = n;
+    }
     cluster.sync();
-    if (slice == 0)
-      for (int q = 1; q < slices; ++q) merge(s, cluster.map_shared_rank(&part, q)->s);
+    if (slice != 0) return;
+    const int q = lane % kMaxSlices;
+    s.x = q < slices ? parts.x[q] : -INFINITY;
+    s.l = q < slices ? parts.l[q] : 0.f;
+    s.w = q < slices ? parts.w[q] : 0.f;
+    s = across(s, kMaxSlices / 2);
   } else {
+    if (tid == 0) parts.n[0] = n;
     __syncthreads();
   }
-  if (slice == 0) {
-    const float lz = logf(s.l);  // ln Z
-    if (tid == 0) {
-      if (a.logprob) {
-        const uint32_t t = a.targets[r];
-        float lp = NAN;
-        if (t < uint64_t(a.V)) lp = (row[t] - s.x) - lz;
-        else if (a.err) atomicCAS(a.err, 0, kErrToken);
-        a.logprob[r] = lp;
-      }
-      if (a.entropy) a.entropy[r] = lz - s.w / s.l * kLn2;
+  const float lz = logf(s.l);  // ln Z
+  if (tid == 0) {
+    if (a.logprob) {
+      float lp = NAN;
+      if (target < uint32_t(V)) lp = (at_target - s.x) - lz;
+      else if (a.err) atomicCAS(a.err, 0, kErrToken);
+      a.logprob[r] = lp;
     }
-    for (int i = tid; i < slices * a.n_top; i += kThreads) {
-      const int q = i / a.n_top, j = i - q * a.n_top;
-      const Part* own = slices > 1 ? cluster.map_shared_rank(&part, q) : &part;
-      if (j >= own->n) continue;
-      const u64 k = own->top[j];
-      int rank = j;
-      for (int o = 0; o < slices; ++o) {
-        if (o == q) continue;
-        const Part* other = cluster.map_shared_rank(&part, o);
-        int lo = 0, hi = other->n;  // the number of its keys above k
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (other->top[mid] > k) lo = mid + 1;
-          else hi = mid;
-        }
-        rank += lo;
+    if (a.entropy) a.entropy[r] = lz - s.w / s.l * kLn2;
+  }
+#pragma unroll 1
+  for (int i = tid; i < slices * kMaxTopK; i += kThreads) {
+    const int q = i / kMaxTopK, j = i % kMaxTopK;
+    if (j >= parts.n[q]) continue;
+    const u64 k = parts.top[q][j];
+    int rank = j;
+#pragma unroll 1
+    for (int o = 0; o < slices; ++o) {
+      if (o == q) continue;
+      int lo = 0, hi = parts.n[o];  // the number of its keys above k
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (parts.top[o][mid] > k) lo = mid + 1;
+        else hi = mid;
       }
-      if (rank < a.n_top) {
-        a.top_ids[r * a.n_top + rank] = ~uint32_t(k);
-        a.top_logprobs[r * a.n_top + rank] = (key_value(k) - s.x) - lz;
-      }
+      rank += lo;
+    }
+    if (rank < a.n_top) {
+      a.top_ids[r * a.n_top + rank] = ~uint32_t(k);
+      a.top_logprobs[r * a.n_top + rank] = (key_value(k) - s.x) - lz;
     }
   }
-  if (slices > 1) cluster.sync();  // no CTA leaves while its part is read
 }
 
 }  // namespace
@@ -336,7 +378,7 @@ cudaError_t launch_logprobs(const LogprobsArgs& a, cudaStream_t s, int num_sms) 
   // Few rows: a cluster of CTAs a row, up to two CTAs an SM in all and no
   // slice below 4 loads a thread.
   int slices = 1;
-  while (slices < 8 && a.rows * slices * 2 <= 2 * num_sms &&
+  while (slices < kMaxSlices && a.rows * slices * 2 <= 2 * num_sms &&
          a.V >= int64_t(slices) * 2 * kThreads * 16)
     slices *= 2;
   cudaLaunchConfig_t cfg = {};
