@@ -3,10 +3,11 @@
 // No counterpart in the reference, whose cache holds f32 rows
 // (src/model.rs:250-332).
 //
-// Both kernels move data: 8 f32 a thread, 4 threads a group of 32 (two of 16
-// for head dim 16), a warp for 256 / d consecutive rows of one head, so a
-// warp reads 1 KB of f32 in segments of d floats and its codes (128 bytes)
-// and parameters (32 or 64) are whole sectors of the cache.
+// Both kernels move data.  A warp's unit is 256 / d consecutive rows of one
+// head: 1 KB of f32 in segments of d floats, and codes (128 bytes) and
+// parameters (32 or 64) that are whole sectors of the cache.  The f32 side
+// goes 16 bytes a lane, a warp's 512 in one piece; 4 units a warp, their loads
+// in flight together, once there are enough rows to fill the GPU so.
 #include "kv4.cuh"
 
 namespace tmg {
@@ -24,120 +25,156 @@ struct Rows {
   int32_t* err;
 };
 
-// A warp's work: rows t0 .. of one head of one stream, keys or values.
+// A warp's work: U units from row t0 of one head of one stream, keys or values.
 struct Work {
   bool value;
   int h, m;
   int64_t t0;
 };
-template <int D>
-__device__ __forceinline__ bool warp_work(const Rows& a, int64_t w, Work* o) {
-  const int64_t nt = (a.T + 256 / D - 1) / (256 / D);
-  const int n = 2 * a.kv.nkv;
-  const int c = int(w % n);
+template <int D, int U>
+__device__ __forceinline__ bool warp_work(const Rows& a, Work* o) {
+  constexpr int R = 256 / D * U;  // rows
+  const unsigned nt = unsigned((a.T + R - 1) / R), n = 2u * a.kv.nkv;
+  unsigned w = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+  const unsigned c = w % n;
   w /= n;
-  o->value = c >= a.kv.nkv;
-  o->h = o->value ? c - a.kv.nkv : c;
-  o->t0 = w % nt * (256 / D);
-  w /= nt;
-  o->m = int(w);
-  return w < a.kv.M;
+  o->value = int(c) >= a.kv.nkv;
+  o->h = o->value ? int(c) - a.kv.nkv : int(c);
+  o->t0 = int64_t(w % nt) * R;
+  o->m = int(w / nt);
+  return o->m < a.kv.M;
 }
 
-// The row of this thread and whether it takes part; its cache row.
-template <int D>
-__device__ __forceinline__ bool thread_row(const Rows& a, const Work& w, int lane, int64_t* t,
-                                           int64_t* crow) {
-  *t = w.t0 + lane / (D / 8);
-  int64_t n = a.T;
-  if (a.count) n = min(n, int64_t(max(a.count[w.m], 0)));
-  if (*t >= n) return false;
-  const int64_t p = int64_t(a.pos[w.m]) + *t;
+// Rows of stream m that are no padding, and the first one's position.
+__device__ __forceinline__ int64_t row_count(const Rows& a, int m) {
+  return a.count ? min(a.T, int64_t(max(a.count[m], 0))) : a.T;
+}
+// The cache row of position p, or -1 (reported) outside the cache.
+__device__ __forceinline__ int64_t cache_row(const Rows& a, const Work& w, int64_t p) {
   if (p < 0 || p >= a.kv.cap) {
     if (a.err) atomicCAS(a.err, 0, kErrPosition);
-    return false;
+    return -1;
   }
-  *crow = (int64_t(w.m) * a.kv.nkv + w.h) * a.kv.cap + p;
-  return true;
+  return (int64_t(w.m) * a.kv.nkv + w.h) * a.kv.cap + p;
 }
 
-template <int D>
+// 8 elements a lane: a group's arithmetic (a division among it) is repeated
+// by 4 lanes and not by 8.
+template <int D, int U>
 __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const Rows a) {
   constexpr int G = D < 32 ? D : 32, LG = G / 8;  // lanes a group
   Work w;
   const int lane = threadIdx.x & 31;
-  if (!warp_work<D>(a, int64_t(blockIdx.x) * (kThreads / 32) + threadIdx.x / 32, &w)) return;
-  int64_t t, crow;
-  const bool on = thread_row<D>(a, w, lane, &t, &crow);
-  const int e = lane % (D / 8) * 8;  // first element of the head's row
-  float x[8] = {};
-  if (on) {
-    const float* p = (w.value ? a.v_in : a.k_in) + (int64_t(w.m) * a.T + t) * a.ld + w.h * D + e;
-    const float4 u = __ldg(reinterpret_cast<const float4*>(p));
-    const float4 v = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-    x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
-  }
-  float lo = x[0], hi = x[0];
-  bool ok = true;
+  if (!warp_work<D, U>(a, &w)) return;
+  const int64_t n = row_count(a, w.m), p0 = a.pos[w.m];
+  const float* in = (w.value ? a.v_in : a.k_in) + int64_t(w.m) * a.T * a.ld + w.h * D;
+  const int t0 = lane * 8 / D, e = lane * 8 % D;  // the lane's row of a unit, and column
+  float4 v[U][2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    ok = ok && fabsf(x[i]) <= 3.402823466e38f;
+  for (int i = 0; i < U; ++i) {
+    const int64_t t = w.t0 + i * (256 / D) + t0;
+    v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (t < n) {
+      const float4* p = reinterpret_cast<const float4*>(in + t * a.ld + e);
+      v[i][0] = __ldg(p);
+      v[i][1] = __ldg(p + 1);
+    }
   }
-#pragma unroll
-  for (int o = 1; o < LG; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    ok = __shfl_xor_sync(0xffffffffu, int(ok), o) && ok;
-  }
-  const uint32_t word = kv4_params(lo, hi, ok);
-  const float m = kv4_min(word), s = kv4_step(word), inv = 1.0f / s;
-  uint32_t codes = 0;
-  if (s == s)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) codes |= kv4_code(x[i], m, s, inv) << (4 * i);
-  if (!on) return;
   uint8_t* cb = w.value ? a.kv.vc : a.kv.kc;
   uint32_t* pb = w.value ? a.kv.vp : a.kv.kp;
-  *reinterpret_cast<uint32_t*>(cb + crow * (D / 2) + e / 2) = codes;
-  if (lane % LG == 0) pb[crow * (D / G) + e / G] = word;
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const float x[8] = {v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w,
+                        v[i][1].x, v[i][1].y, v[i][1].z, v[i][1].w};
+    float lo = x[0], hi = x[0];
+    bool ok = true;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      lo = fminf(lo, x[j]);
+      hi = fmaxf(hi, x[j]);
+      ok = ok && fabsf(x[j]) <= 3.402823466e38f;
+    }
+    // the group's extremes over its lanes; +inf above stands for a value that
+    // is not finite
+    hi = ok ? hi : INFINITY;
+#pragma unroll
+    for (int o = 1; o < LG; o <<= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    const uint32_t word = kv4_params(lo, hi, hi < INFINITY);
+    const uint32_t codes = kv4_codes(x, word);
+    const int64_t t = w.t0 + i * (256 / D) + t0;
+    const int64_t row = t < n ? cache_row(a, w, p0 + t) : -1;
+    if (row < 0) continue;
+    *reinterpret_cast<uint32_t*>(cb + row * (D / 2) + e / 2) = codes;
+    if (lane % LG == 0) pb[row * (D / G) + e / G] = word;
+  }
 }
 
-template <int D>
+// The f32 side in pieces of 128 elements, 4 a lane: element 4 lane of piece i
+// is in row (128 i + 4 lane) / d of the warp's, column (128 i + 4 lane) % d.
+template <int D, int U>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const Rows a) {
   constexpr int G = D < 32 ? D : 32;
   Work w;
   const int lane = threadIdx.x & 31;
-  if (!warp_work<D>(a, int64_t(blockIdx.x) * (kThreads / 32) + threadIdx.x / 32, &w)) return;
-  float* ob = w.value ? a.v_out : a.k_out;
-  int64_t t, crow;
-  if (ob == nullptr || !thread_row<D>(a, w, lane, &t, &crow)) return;
-  const int e = lane % (D / 8) * 8;
+  if (!warp_work<D, U>(a, &w)) return;
+  float* out = w.value ? a.v_out : a.k_out;
+  if (out == nullptr) return;
+  const int64_t n = row_count(a, w.m), p0 = a.pos[w.m];
   const uint8_t* cb = w.value ? a.kv.vc : a.kv.kc;
   const uint32_t* pb = w.value ? a.kv.vp : a.kv.kp;
-  const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(cb + crow * (D / 2) + e / 2));
-  const uint32_t word = __ldg(pb + crow * (D / G) + e / G);
-  const float m = kv4_min(word), s = kv4_step(word);
-  float x[8];
+  // codes 8 a lane, as whole sectors
+  uint32_t c[U], word[U];
+  bool on[U];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = fmaf(float((c >> (4 * i)) & 15u), s, m);
-  float4* p = reinterpret_cast<float4*>(ob + (int64_t(w.m) * a.T + t) * a.ld + w.h * D + e);
-  p[0] = make_float4(x[0], x[1], x[2], x[3]);
-  p[1] = make_float4(x[4], x[5], x[6], x[7]);
+  for (int i = 0; i < U; ++i) {
+    const int e = i * 256 + lane * 8;
+    const int64_t t = w.t0 + e / D;
+    const int64_t row = t < n ? cache_row(a, w, p0 + t) : -1;
+    on[i] = row >= 0;
+    c[i] = word[i] = 0;
+    if (on[i]) {
+      c[i] = __ldg(reinterpret_cast<const uint32_t*>(cb + row * (D / 2) + e % D / 2));
+      word[i] = __ldg(pb + row * (D / G) + e % D / G);
+    }
+  }
+  out += int64_t(w.m) * a.T * a.ld + w.h * D;
+#pragma unroll
+  for (int i = 0; i < 2 * U; ++i) {
+    // 4 of the 8 codes that lane 16 (i % 2) + lane / 2 has loaded
+    const int src = 16 * (i % 2) + lane / 2;
+    const uint32_t cc = __shfl_sync(0xffffffffu, c[i / 2], src) >> (16 * (lane & 1));
+    const uint32_t ww = __shfl_sync(0xffffffffu, word[i / 2], src);
+    if (!__shfl_sync(0xffffffffu, int(on[i / 2]), src)) continue;
+    const float m = kv4_min(ww), s = kv4_step(ww);
+    const int e = i * 128 + lane * 4;
+    __stcs(reinterpret_cast<float4*>(out + (w.t0 + e / D) * a.ld + e % D),
+           make_float4(fmaf(float(cc & 15u), s, m), fmaf(float((cc >> 4) & 15u), s, m),
+                       fmaf(float((cc >> 8) & 15u), s, m), fmaf(float((cc >> 12) & 15u), s, m)));
+  }
+}
+
+template <int D, int U>
+cudaError_t launch_units(const Rows& a, bool append, cudaStream_t s) {
+  const int64_t warps = 2ll * a.kv.M * a.kv.nkv * ((a.T + 256 / D * U - 1) / (256 / D * U));
+  const int64_t blocks = (warps + kThreads / 32 - 1) / (kThreads / 32);
+  if (blocks > INT32_MAX / (kThreads / 32)) return cudaErrorInvalidValue;
+  if (append)
+    kv4_append_kernel<D, U><<<unsigned(blocks), kThreads, 0, s>>>(a);
+  else
+    kv4_read_kernel<D, U><<<unsigned(blocks), kThreads, 0, s>>>(a);
+  return cudaGetLastError();
 }
 
 template <int D>
 cudaError_t launch_rows(const Rows& a, bool append, cudaStream_t s) {
-  const int64_t warps = 2ll * a.kv.M * a.kv.nkv * ((a.T + 256 / D - 1) / (256 / D));
-  const int64_t blocks = (warps + kThreads / 32 - 1) / (kThreads / 32);
-  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  if (append)
-    kv4_append_kernel<D><<<unsigned(blocks), kThreads, 0, s>>>(a);
-  else
-    kv4_read_kernel<D><<<unsigned(blocks), kThreads, 0, s>>>(a);
-  return cudaGetLastError();
+  // several units a warp from about two waves of 148 x 64 warps on; 2 to write
+  // (4 took 30 us where 2 take 28), 4 to read
+  const int64_t units = 2ll * a.kv.M * a.kv.nkv * ((a.T + 256 / D - 1) / (256 / D));
+  if (units < 18944) return launch_units<D, 1>(a, append, s);
+  return append ? launch_units<D, 2>(a, append, s) : launch_units<D, 4>(a, append, s);
 }
 
 cudaError_t launch_rows_d(const Rows& a, bool append, cudaStream_t s) {

@@ -35,25 +35,42 @@ __device__ __forceinline__ uint32_t kv4_params(float lo, float hi, bool ok) {
   const uint32_t lb = __float_as_uint(lo);
   uint32_t m = lb & 0xffff0000u;
   if ((lb >> 31) && m != lb) m += 0x10000u;  // towards -inf
-  // the smallest bf16 s with 15 s >= hi - m: each step rounds up, and 15 s
-  // (12 bits) is an f32, so rounding up twice picks no larger one
+  // the smallest bf16 s with 15 s >= hi - m: 15 s (12 bits) is an f32, so the
+  // range may be rounded up first.  A product that is not below range / 15
+  // gives s or the bf16 above it.
   const float range = __fsub_ru(hi, __uint_as_float(m));
-  const uint32_t sb = __float_as_uint(__fdiv_ru(range, 15.0f));
-  const uint32_t s = (sb + 0xffffu) & 0xffff0000u;
+  uint32_t s = (__float_as_uint(__fmul_ru(range, 0x1.111112p-4f)) + 0xffffu) & 0xffff0000u;
+  if (s > 0u && 15.0f * __uint_as_float(s - 0x10000u) >= range) s -= 0x10000u;
   ok = ok && (m & 0x7f800000u) != 0x7f800000u && (s & 0x7f800000u) != 0x7f800000u &&
        range <= 3.402823466e38f;
   return ok ? (m | (s >> 16)) : 0x7fc07fc0u;
 }
 
-// The code of x in a group with parameters (m, s), inv = 1 / s.  The f32
-// quotient is off by less than 4e-6 (three roundings of a value below 16),
-// so it decides except next to a tie; there the 64-bit quotient does.
-__device__ __forceinline__ uint32_t kv4_code(float x, float m, float s, float inv) {
-  const float t = (x - m) * inv;
-  const float r = rintf(t);
-  if (fabsf(fabsf(t - r) - 0.5f) > 1e-5f) return uint32_t(r);
-  if (!(s > 0.0f)) return 0u;
-  return uint32_t(rint((double(x) - double(m)) / double(s)));
+// The 8 codes of x in a group with parameter word `word`, lowest first.  The
+// f32 quotient (x - m) / s is off by less than 4e-6 (15 times 2^-22: the
+// difference, the reciprocal and the product), so it decides except next to a
+// tie, or where 1 / s leaves f32; there the 64-bit quotient does.
+__device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], uint32_t word) {
+  const float m = kv4_min(word), s = kv4_step(word);
+  if (!(s > 0.0f)) return 0u;  // a constant group, or one that stands for NaN
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: a sum's low bits are the rounded t
+  uint32_t codes = 0u;
+  float off = 0.0f;
+#pragma unroll
+  for (int j = 7; j >= 0; --j) {
+    const float t = (x[j] - m) * inv, r = t + kMagic;
+    off = fmaxf(off, fabsf(t - (r - kMagic)));
+    codes = codes * 16u + (__float_as_uint(r) & 15u);
+  }
+  if (off > 0.5f - 1e-5f || s < 0x1p-126f) {
+    codes = 0u;
+#pragma unroll 1
+    for (int j = 7; j >= 0; --j)
+      codes = codes * 16u + uint32_t(rint((double(x[j]) - double(m)) / double(s)));
+  }
+  return codes;
 }
 
 }  // namespace tmg
