@@ -153,6 +153,16 @@ int64_t tmg_weight_bytes(const tmg_ctx* ctx);
  * ------------------------------------------------------------------------ */
 
 int tmg_kv_create(tmg_ctx* ctx, int32_t n_streams, int64_t capacity, tmg_kv** out);
+/* The same cache with its rows in 4 bits, 6.4 times smaller at head_dim >= 32
+ * (no counterpart in the reference): keys after RoPE and values quantised as
+ * they are written, in groups of min(head_dim, 32) elements of a head as
+ * tmg_kv4 below states.  Every attention over it, of the tokens of a prompt
+ * too, sees the rows as the cache holds them, so logits do not depend on how a
+ * prompt is cut into calls beyond rounding.  Takes every call that a tmg_kv
+ * does except tmg_fused_group_init and the trace aids; greedy decode runs the
+ * per-step graph.  One layer and stream of f32 rows is kept beside it for
+ * prefill.  head_dim 16, 32, 64 or 128, at most 16 query heads per kv head. */
+int tmg_kv_create_q4(tmg_ctx* ctx, int32_t n_streams, int64_t capacity, tmg_kv** out);
 int tmg_kv_destroy(tmg_kv* kv);
 /* KvCache::len(layer) for one stream (src/model.rs:283-285). */
 int tmg_kv_len(const tmg_kv* kv, int32_t layer, int32_t stream, int64_t* out);
@@ -180,6 +190,15 @@ int tmg_forward_token(tmg_ctx* ctx, tmg_kv* kv, const uint32_t* tokens, float* l
  * on an empty prompt, model.rs:495-497). */
 int tmg_forward_seq(tmg_ctx* ctx, tmg_kv* kv, int32_t stream, const uint32_t* tokens, int64_t T,
                     float* logits);
+/* tmg_forward_seq with every row scored (no counterpart in the reference):
+ * host outputs, each NULL if not wanted.  logprob[t], t < T - 1: the natural
+ * log of the probability that row t gives tokens[t + 1]; entropy[T]: its
+ * distribution's entropy in nats; top_ids / top_logprobs [T, n_top] (n_top 0 to
+ * 64): the most likely tokens after each row, as tmg_op_logprobs orders them.
+ * The tokens are appended to the stream.  One GPU only. */
+int tmg_score(tmg_ctx* ctx, tmg_kv* kv, int32_t stream, const uint32_t* tokens, int64_t T,
+              int32_t n_top, float* logprob, float* entropy, uint32_t* top_ids,
+              float* top_logprobs);
 /* generate, src/model.rs:614-663, for stream 0 of `kv` (reset first):
  * prefill, then up to max_tokens steps of penalty -> argmax/sample -> EOS
  * check -> forward_token, all on the device.  tokens_out[max_tokens];

@@ -109,6 +109,7 @@ unsafe extern "C" {
 
     // KV cache
     pub fn tmg_kv_create(ctx: *mut TmgCtx, n_streams: i32, capacity: i64, out: *mut *mut TmgKv) -> i32;
+    pub fn tmg_kv_create_q4(ctx: *mut TmgCtx, n_streams: i32, capacity: i64, out: *mut *mut TmgKv) -> i32;
     pub fn tmg_kv_destroy(kv: *mut TmgKv) -> i32;
     pub fn tmg_kv_len(kv: *const TmgKv, layer: i32, stream: i32, out: *mut i64) -> i32;
     pub fn tmg_kv_reset(kv: *mut TmgKv) -> i32;
@@ -119,6 +120,9 @@ unsafe extern "C" {
     pub fn tmg_forward_token(ctx: *mut TmgCtx, kv: *mut TmgKv, tokens: *const u32, logits: *mut f32) -> i32;
     pub fn tmg_forward_seq(ctx: *mut TmgCtx, kv: *mut TmgKv, stream: i32, tokens: *const u32, t: i64,
                            logits: *mut f32) -> i32;
+    pub fn tmg_score(ctx: *mut TmgCtx, kv: *mut TmgKv, stream: i32, tokens: *const u32, t: i64,
+                     n_top: i32, logprob: *mut f32, entropy: *mut f32, top_ids: *mut u32,
+                     top_logprobs: *mut f32) -> i32;
     pub fn tmg_generate(ctx: *mut TmgCtx, kv: *mut TmgKv, prompt: *const u32, t: i64,
                         params: *const TmgGenParams, uniforms: *const f32, tokens_out: *mut u32,
                         n_out: *mut i64, first_logits: *mut f32, prefill_secs: *mut f64,

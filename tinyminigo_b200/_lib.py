@@ -100,6 +100,7 @@ SIGNATURES = {
     "tmg_finalize": (_I, [_P]),
     "tmg_weight_bytes": (_I64, [_P]),
     "tmg_kv_create": (_I, [_P, _I32, _I64, _PP]),
+    "tmg_kv_create_q4": (_I, [_P, _I32, _I64, _PP]),
     "tmg_kv_destroy": (_I, [_P]),
     "tmg_kv_len": (_I, [_P, _I32, _I32, _PI64]),
     "tmg_kv_reset": (_I, [_P]),
@@ -107,6 +108,7 @@ SIGNATURES = {
     "tmg_kv_read": (_I, [_P, _I32, _I32, _P, _P]),
     "tmg_forward_token": (_I, [_P, _P, _P, _P]),
     "tmg_forward_seq": (_I, [_P, _P, _I32, _P, _I64, _P]),
+    "tmg_score": (_I, [_P, _P, _I32, _P, _I64, _I32, _P, _P, _P, _P]),
     "tmg_generate": (_I, [_P, _P, _P, _I64, ctypes.POINTER(GenParamsC), _P, _P, _PI64, _P,
                           ctypes.POINTER(ctypes.c_double), TOKEN_CB, _P]),
     "tmg_generate_batch": (_I, [_P, _P, _P, _I64, ctypes.POINTER(GenParamsC), _P, _P, _PI64]),

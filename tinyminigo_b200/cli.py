@@ -4,7 +4,7 @@ library: the same flags and defaults, the same flow.
     python -m tinyminigo_b200 -m dir/model.safetensors --template chat.jinja \\
         [--tokenizer tokenizer.json] [--max-tokens 256] [--temperature 0] \\
         [--top-k 0] [--top-p 1] [--repetition-penalty 1] [--seed 42] \\
-        [--dump-first-logits out.json] [--repack out.tmb] "prompt"
+        [--kv-bits 32|4] [--dump-first-logits out.json] [--repack out.tmb] "prompt"
 
 `--repack` writes a TMB1 file and exits (src/main.rs:29-35); otherwise the
 model goes to HBM (a TMB1 file or safetensors + config.json), the prompt is
@@ -50,6 +50,8 @@ def parse_args(argv=None) -> argparse.Namespace:
                     help="Repetition penalty (1.0 = disabled)")
     ap.add_argument("--seed", metavar="SEED", type=int, default=42,
                     help="Random seed for sampling")
+    ap.add_argument("--kv-bits", metavar="B", type=int, default=32, choices=(4, 32),
+                    help="Bits of a KV cache element: 32, or 4 (not in the reference)")
     ap.add_argument("prompt", help="The user prompt")
     ap.add_argument("--dump-first-logits", metavar="FILE", default=None,
                     help=argparse.SUPPRESS)
@@ -148,7 +150,10 @@ def _run(args) -> int:
         sys.stdout.flush()
 
     t_start = time.perf_counter()
-    res = generate(m, ids, params, on_token=on_token)
+    cache = None
+    if args.kv_bits == 4:
+        cache = m.new_cache(len(ids) + args.max_tokens + 1, bits=4)
+    res = generate(m, ids, params, on_token=on_token, cache=cache)
     if args.dump_first_logits is not None:
         Path(args.dump_first_logits).write_text(first_logits_dump(res.logits_first_step))
     print()

@@ -130,6 +130,9 @@ struct tmg_ctx {
   // BF16 parts of q, k and v^T for the tensor-core prefill attention
   void* pfa = nullptr;
   size_t pfa_cap = 0;
+  // logits and scores of tmg_score
+  void* sc_buf = nullptr;
+  size_t sc_cap = 0;
   // pinned staging
   void* pinned = nullptr;
   size_t pinned_cap = 0;
@@ -173,6 +176,15 @@ struct tmg_kv {
   int64_t cap = 0;
   int kvd = 0;
   std::vector<float*> k, v;  // per layer [M, cap, kvd]
+  // a 4-bit cache (tmg_kv_create_q4) instead: per layer codes and parameters,
+  // the streams' lengths of a step, the attention's workspace, one layer and
+  // stream of f32 rows that a prefill's attention reads, and its position
+  bool q4 = false;
+  std::vector<Kv4> q;
+  int32_t* q_lens = nullptr;
+  void* q_ws = nullptr;
+  float *q_k = nullptr, *q_v = nullptr;
+  int32_t* q_pos = nullptr;  // [0]: 0, [1]: a prefill chunk's first position
   float *rope_cos = nullptr, *rope_sin = nullptr;
   int32_t* d_state = nullptr;  // token | pos | done | n_gen, kMaxStreams each
   StreamState st{};
@@ -199,6 +211,7 @@ struct tmg_kv {
 namespace {
 
 constexpr int64_t kPrefillChunk = 4096;
+constexpr int64_t kScoreRows = 256;  // rows of logits at a time (131 MB at 128256 tokens)
 
 // Why the last tmg_create on this thread failed (there is no context to hold it).
 thread_local std::string g_create_err;
@@ -660,6 +673,19 @@ cudaError_t ensure_split(tmg_ctx* c, size_t n) {
   return cudaSuccess;
 }
 
+// One stream of a 4-bit cache.
+Kv4 kv4_stream(const Kv4& kv, int m) {
+  Kv4 o = kv;
+  const size_t row = size_t(m) * kv.nkv * kv.cap;
+  const int per = kv.d < 32 ? kv.d : 32;
+  o.kc += row * (kv.d / 2);
+  o.vc += row * (kv.d / 2);
+  o.kp += row * (kv.d / per);
+  o.vp += row * (kv.d / per);
+  o.M = 1;
+  return o;
+}
+
 // Causal prefill attention of T query rows at pos0.. over cache rows
 // [0, pos0 + T): the tcgen05 kernel for head dim 64 (TMG_PREFILL_ATTN=simt
 // keeps the CUDA-core kernel), else the CUDA-core one.
@@ -899,8 +925,8 @@ cudaError_t enqueue_forward(tmg_ctx* c, tmg_kv* kv, const StreamState& st, bool 
     AttnDecodeArgs T;
     T.qkv = c->qkv;
     T.qkv_ld = c->qkv_rows;
-    T.kc = kv->k[l];
-    T.vc = kv->v[l];
+    T.kc = kv->q4 ? nullptr : kv->k[l];
+    T.vc = kv->q4 ? nullptr : kv->v[l];
     T.cap = kv->cap;
     T.rope_cos = kv->rope_cos;
     T.rope_sin = kv->rope_sin;
@@ -917,7 +943,26 @@ cudaError_t enqueue_forward(tmg_ctx* c, tmg_kv* kv, const StreamState& st, bool 
     T.err = c->d_err;
     T.trace = tc.take(1);
     B();
-    TMG_CUDA_TRY(launch_attn_decode(T, c->stream, pdl));
+    if (kv->q4) {
+      TMG_CUDA_TRY(launch_kv4_step(kv->q[l], c->qkv, c->qkv_rows, c->nq, st, kv->rope_cos,
+                                   kv->rope_sin, int(kv->cap), kv->q_lens, c->stream, pdl));
+      AttnKv4Args Q;
+      Q.kv = kv->q[l];
+      Q.q = c->qkv;
+      Q.q_ld = c->qkv_rows;
+      Q.lens = kv->q_lens;
+      Q.max_len = kv->cap;
+      Q.nq = c->nq;
+      Q.scale = T.scale;
+      Q.out = c->attn;
+      Q.out_ld = int64_t(c->nq) * c->d;
+      Q.ws = kv->q_ws;
+      Q.err = c->d_err;
+      Q.num_sms = c->num_sms;
+      TMG_CUDA_TRY(launch_attn_kv4(Q, c->stream, pdl));
+    } else {
+      TMG_CUDA_TRY(launch_attn_decode(T, c->stream, pdl));
+    }
     E(1);
     GemvArgs O;
     O.w = Lw.wo;
@@ -1015,11 +1060,21 @@ cudaError_t enqueue_forward(tmg_ctx* c, tmg_kv* kv, const StreamState& st, bool 
   return cudaSuccess;
 }
 
+// Scores of the rows of a forward_seq (tmg_score): host outputs, each may be
+// null; logprob[t] of the token after row t.
+struct Scores {
+  int n_top = 0;
+  float *logprob = nullptr, *entropy = nullptr, *top_logprobs = nullptr;
+  uint32_t* top_ids = nullptr;
+};
+int score_rows(tmg_ctx* c, const uint32_t* tokens, int64_t t0, int64_t Tc, int64_t T,
+               const Scores& out);
+
 // forward_seq for one stream (model.rs:503-590): chunks of kPrefillChunk
 // tokens through all layers; the last row's logits land in row `stream` of
 // the decode logits buffer.
 int forward_seq(tmg_ctx* c, tmg_kv* kv, int stream, const uint32_t* tokens, int64_t T,
-                bool host_tokens) {
+                bool host_tokens, const Scores* scores = nullptr) {
   int rc;
   if ((rc = ensure_prefill(c, T))) return rc;
   const int64_t p0 = kv->lens[stream];
@@ -1042,14 +1097,19 @@ int forward_seq(tmg_ctx* c, tmg_kv* kv, int stream, const uint32_t* tokens, int6
       dtok = tokens + t0;
     }
     CK(launch_embed(c->embed, dtok, Tc, c->h, c->X, c->stream), "embed");
+    if (kv->q4) {
+      StreamState q{};
+      q.pos = kv->q_pos;
+      CK(launch_set_pos(q, 1, int32_t(pos0), c->stream), "set pos");
+    }
     for (int l = 0; l < c->L; ++l) {
       const Layer& Lw = c->layers[l];
       // one profiler range per layer of the chunk (host side: the enqueues)
       char rname[48];
       std::snprintf(rname, sizeof rname, "prefill layer %d", l);
       NvtxRange layer_range(rname);
-      float* kc = kv->k[l] + size_t(stream) * kv->cap * kvd;
-      float* vc = kv->v[l] + size_t(stream) * kv->cap * kvd;
+      float* kc = kv->q4 ? kv->q_k : kv->k[l] + size_t(stream) * kv->cap * kvd;
+      float* vc = kv->q4 ? kv->q_v : kv->v[l] + size_t(stream) * kv->cap * kvd;
       if (!c->i8 && gemm_tc_supported(c->h, Lw.wqkv)) {
         // rmsnorm written straight as the qkv GEMM's hi/lo operands
         CK(ensure_split(c, size_t(Tc) * c->h), "split");
@@ -1073,11 +1133,21 @@ int forward_seq(tmg_ctx* c, tmg_kv* kv, int stream, const uint32_t* tokens, int6
       bool att_parts = false, roped = false;
       const bool tc_attn = attn_prefill_tc_ok(c->QKV, c->qkv_rows, kc, vc, Tc, pos0, c->nq, c->nkv,
                                               c->d, c->ATT, qd) &&
-                           !prefill_attn_simt();
+                           !prefill_attn_simt() && !kv->q4;
       if (!tc_attn)
         CK(launch_rope_append(c->QKV, c->qkv_rows, Tc, c->nq, c->nkv, c->d, kv->rope_cos,
                               kv->rope_sin, pos0, kc, vc, c->stream),
            "rope");
+      if (kv->q4) {
+        // the chunk's rows quantised, and all rows read back as what the cache
+        // stands for, so that the attention sees what later steps will see
+        const Kv4 qs = kv4_stream(kv->q[l], stream);
+        CK(launch_kv4_append(qs, kc + pos0 * kvd, vc + pos0 * kvd, kvd, Tc, kv->q_pos + 1, nullptr,
+                             c->d_err, c->stream),
+           "kv4 append");
+        CK(launch_kv4_read(qs, kv->q_pos, nullptr, pos0 + Tc, kc, vc, kvd, c->d_err, c->stream),
+           "kv4 read");
+      }
       CK(prefill_attention(c, c->QKV, c->qkv_rows, kc, vc, Tc, pos0, scale, c->ATT, qd, c->nq,
                            c->nkv, c->d, o_parts ? c->sp_hi : nullptr,
                            o_parts ? c->sp_lo : nullptr, &att_parts,
@@ -1157,6 +1227,7 @@ int forward_seq(tmg_ctx* c, tmg_kv* kv, int stream, const uint32_t* tokens, int6
       }
       if (tp) CK(tp_reduce_add(c, c->Xn, c->X, Tc * c->h), "allreduce");
     }
+    if (scores && (rc = score_rows(c, tokens, t0, Tc, T, *scores))) return rc;
     if (t0 + Tc == T) {
       GemvArgs H;
       H.w = c->lm_head;
@@ -1178,6 +1249,82 @@ int forward_seq(tmg_ctx* c, tmg_kv* kv, int stream, const uint32_t* tokens, int6
   }
   CK(launch_set_pos(kv->st, stream, int32_t(p0 + T), c->stream), "set pos");
   kv->lens[stream] = p0 + T;
+  return TMG_OK;
+}
+
+// The chunk's final hidden rows (c->X, Tc of them from row t0 of T) through
+// the final norm and the LM head, kScoreRows at a time, and the rows' scores
+// to the host.
+int score_rows(tmg_ctx* c, const uint32_t* tokens, int64_t t0, int64_t Tc, int64_t T,
+               const Scores& out) {
+  const int64_t R = std::min<int64_t>(kScoreRows, c->pf_cap);
+  const size_t per = 3 + 2 * size_t(out.n_top);  // a row's target, logprob, entropy, alternatives
+  const size_t need = size_t(R) * c->V * 4 + size_t(Tc) * per * 4;
+  if (c->sc_cap < need) {
+    CK(cudaStreamSynchronize(c->stream), "score");
+    if (c->sc_buf) cudaFree(c->sc_buf);
+    c->sc_buf = nullptr;
+    c->sc_cap = 0;
+    CK(cudaMalloc(&c->sc_buf, need), "score scratch");
+    c->sc_cap = need;
+  }
+  float* logits = static_cast<float*>(c->sc_buf);
+  uint32_t* target = reinterpret_cast<uint32_t*>(logits + size_t(R) * c->V);
+  float* logprob = reinterpret_cast<float*>(target + Tc);
+  float* entropy = logprob + Tc;
+  uint32_t* ids = reinterpret_cast<uint32_t*>(entropy + Tc);
+  float* tops = reinterpret_cast<float*>(ids + Tc * out.n_top);
+  // the token after each row; the last row of all has none (any id serves)
+  std::vector<uint32_t> next(tokens + t0, tokens + t0 + Tc);
+  for (int64_t i = 0; i < Tc; ++i) next[i] = t0 + i + 1 < T ? tokens[t0 + i + 1] : 0;
+  CK(copy_sync(c, target, next.data(), size_t(Tc) * 4, cudaMemcpyHostToDevice), "score targets");
+  for (int64_t i = 0; i < Tc; i += R) {
+    const int64_t n = std::min(R, Tc - i);
+    const float* x = c->X + size_t(i) * c->h;
+    if (gemm_tc_supported(c->h, c->lm_head)) {
+      CK(ensure_split(c, size_t(n) * c->h), "split");
+      CK(launch_rmsnorm_split(x, c->final_norm, c->cfg.rms_norm_eps, c->h, n, c->sp_hi, c->sp_lo,
+                              c->stream),
+         "rmsnorm");
+      CK(launch_gemm_tc(c->sp_hi, c->sp_lo, c->lm_head, n, c->V, c->h, logits, c->V, false,
+                        c->d_err, c->stream),
+         "lm_head");
+    } else {
+      CK(launch_rmsnorm(x, c->final_norm, c->cfg.rms_norm_eps, c->h, n, 1, c->Xn, c->stream),
+         "rmsnorm");
+      CK(gemm(c, c->Xn, c->lm_head, n, c->V, c->h, logits, c->V, false), "lm_head");
+    }
+    LogprobsArgs a;
+    a.logits = logits;
+    a.ld = a.V = c->V;
+    a.rows = n;
+    a.targets = target + i;
+    a.logprob = logprob + i;
+    a.entropy = entropy + i;
+    a.n_top = out.n_top;
+    a.top_ids = ids + i * out.n_top;
+    a.top_logprobs = tops + i * out.n_top;
+    a.err = c->d_err;
+    CK(launch_logprobs(a, c->stream, c->num_sms), "logprobs");
+  }
+  const int64_t with_next = std::min(Tc, T - 1 - t0);
+  if (out.logprob && with_next > 0)
+    CK(cudaMemcpyAsync(out.logprob + t0, logprob, size_t(with_next) * 4, cudaMemcpyDeviceToHost,
+                       c->stream),
+       "scores");
+  if (out.entropy)
+    CK(cudaMemcpyAsync(out.entropy + t0, entropy, size_t(Tc) * 4, cudaMemcpyDeviceToHost,
+                       c->stream),
+       "scores");
+  if (out.n_top) {
+    CK(cudaMemcpyAsync(out.top_ids + t0 * out.n_top, ids, size_t(Tc) * out.n_top * 4,
+                       cudaMemcpyDeviceToHost, c->stream),
+       "scores");
+    CK(cudaMemcpyAsync(out.top_logprobs + t0 * out.n_top, tops, size_t(Tc) * out.n_top * 4,
+                       cudaMemcpyDeviceToHost, c->stream),
+       "scores");
+  }
+  CK(cudaStreamSynchronize(c->stream), "score");
   return TMG_OK;
 }
 
@@ -1612,7 +1759,7 @@ int tmg_create(int device, const tmg_config* cfg, tmg_ctx** out) {
       run("fused_prepare", fused_prepare()) && run("sample_prepare", sample_prepare()) &&
       run("gemv_i8_prepare", gemv_i8_prepare()) && run("attn_tma_prepare", attn_tma_prepare()) &&
       run("attn_prefill_tc_prepare", attn_prefill_tc_prepare()) &&
-      run("attn_kv4_prepare", attn_kv4_prepare()) &&
+      run("attn_kv4_prepare", attn_kv4_prepare()) && run("kv4_prepare", kv4_prepare()) &&
       run("error word", dalloc(c->allocs, &c->d_err, 4)) && run("error word", zero_sync(c, c->d_err, 16));
   if (step) {
     g_create_err = std::string("tmg_create: ") + step + ": " + cudaGetErrorString(ce);
@@ -1644,7 +1791,7 @@ int tmg_destroy(tmg_ctx* c) {
   for (void* p : {(void*)c->X, (void*)c->Xn, (void*)c->QKV, (void*)c->ATT, (void*)c->G,
                   (void*)c->U, (void*)c->d_tok, c->op_buf, (void*)c->sp_hi, (void*)c->sp_lo, c->pfa,
                   (void*)c->sa_hi, (void*)c->sa_lo,
-                  (void*)c->dq, (void*)c->i8acc})
+                  (void*)c->dq, (void*)c->i8acc, c->sc_buf})
     if (p) cudaFree(p);
   if (c->pinned) cudaFreeHost(c->pinned);
   for (tmg_wmat* m : c->wmats) {
@@ -1758,7 +1905,7 @@ int tmg_finalize(tmg_ctx* c) {
 
 int64_t tmg_weight_bytes(const tmg_ctx* c) { return c ? c->weight_bytes : 0; }
 
-int tmg_kv_create(tmg_ctx* c, int32_t n_streams, int64_t capacity, tmg_kv** out) {
+static int kv_create(tmg_ctx* c, int32_t n_streams, int64_t capacity, bool q4, tmg_kv** out) {
   if (!c || !out || n_streams < 1 || n_streams > kMaxStreams || capacity < 1)
     return fail(c, TMG_ERR_INVALID, "bad KV cache shape (1..16 streams)");
   if (!c->finalized) return fail(c, TMG_ERR_INVALID, "weights not finalized");
@@ -1775,7 +1922,32 @@ int tmg_kv_create(tmg_ctx* c, int32_t n_streams, int64_t capacity, tmg_kv** out)
     return cuda_fail(c, e, "KV cache allocation");
   };
   cudaError_t e;
-  for (int l = 0; l < c->L; ++l) {
+  kv->q4 = q4;
+  if (q4) {
+    Kv4 q;
+    q.M = n_streams;
+    q.nkv = c->nkv;
+    q.d = c->d;
+    q.cap = (capacity + 3) / 4 * 4;
+    const size_t rows = size_t(n_streams) * c->nkv * q.cap;
+    const size_t codes = rows * (c->d / 2), params = rows * (c->d / std::min(c->d, 32));
+    for (int l = 0; l < c->L; ++l) {
+      if ((e = dalloc(kv->allocs, &q.kc, codes)) != cudaSuccess) return bail(e);
+      if ((e = dalloc(kv->allocs, &q.vc, codes)) != cudaSuccess) return bail(e);
+      if ((e = dalloc(kv->allocs, &q.kp, params)) != cudaSuccess) return bail(e);
+      if ((e = dalloc(kv->allocs, &q.vp, params)) != cudaSuccess) return bail(e);
+      kv->q.push_back(q);
+    }
+    if ((e = dalloc(kv->allocs, &kv->q_lens, n_streams)) != cudaSuccess) return bail(e);
+    char* ws = nullptr;
+    if ((e = dalloc(kv->allocs, &ws, attn_kv4_ws(q, c->nq, c->num_sms))) != cudaSuccess) return bail(e);
+    kv->q_ws = ws;
+    if ((e = dalloc(kv->allocs, &kv->q_k, size_t(capacity) * kv->kvd)) != cudaSuccess) return bail(e);
+    if ((e = dalloc(kv->allocs, &kv->q_v, size_t(capacity) * kv->kvd)) != cudaSuccess) return bail(e);
+    if ((e = dalloc(kv->allocs, &kv->q_pos, 2)) != cudaSuccess) return bail(e);
+    if ((e = zero_sync(c, kv->q_pos, 8)) != cudaSuccess) return bail(e);
+  }
+  for (int l = 0; l < c->L && !q4; ++l) {
     float *kp, *vp;
     if ((e = dalloc(kv->allocs, &kp, size_t(n_streams) * capacity * kv->kvd)) != cudaSuccess) return bail(e);
     if ((e = dalloc(kv->allocs, &vp, size_t(n_streams) * capacity * kv->kvd)) != cudaSuccess) return bail(e);
@@ -1799,7 +1971,7 @@ int tmg_kv_create(tmg_ctx* c, int32_t n_streams, int64_t capacity, tmg_kv** out)
   kv->st.gen_cap = 0;
   kv->st.n_eos = 0;
   kv->nsplit = attn_decode_nsplit(c->nkv, n_streams, capacity, c->num_sms);
-  if (c->fused_ok && n_streams == 1) {
+  if (c->fused_ok && n_streams == 1 && !q4) {
     std::vector<FusedLayer> fl(c->L);
     for (int l = 0; l < c->L; ++l) {
       const Layer& Lw = c->layers[l];
@@ -1821,6 +1993,21 @@ int tmg_kv_create(tmg_ctx* c, int32_t n_streams, int64_t capacity, tmg_kv** out)
   c->kvs.push_back(kv);
   *out = kv;
   return TMG_OK;
+}
+
+int tmg_kv_create(tmg_ctx* c, int32_t n_streams, int64_t capacity, tmg_kv** out) {
+  return kv_create(c, n_streams, capacity, false, out);
+}
+
+int tmg_kv_create_q4(tmg_ctx* c, int32_t n_streams, int64_t capacity, tmg_kv** out) {
+  if (c && c->finalized) {
+    if (c->d != 16 && c->d != 32 && c->d != 64 && c->d != 128)
+      return fail(c, TMG_ERR_INVALID, "a 4-bit cache needs head_dim 16, 32, 64 or 128");
+    if (c->nq / c->nkv > 16)
+      return fail(c, TMG_ERR_INVALID, "a 4-bit cache takes at most 16 query heads per kv head");
+  }
+  if (capacity > INT32_MAX - 4) return fail(c, TMG_ERR_INVALID, "capacity beyond 2^31");
+  return kv_create(c, n_streams, capacity, true, out);
 }
 
 // Free a KV cache's device resources (its context is current and alive).
@@ -1895,6 +2082,16 @@ int tmg_kv_read(tmg_kv* kv, int32_t layer, int32_t stream, float* keys, float* v
   cudaSetDevice(c->device);
   CK(cudaStreamSynchronize(c->stream), "kv read");
   const size_t n = size_t(kv->lens[stream]) * kv->kvd;
+  if (kv->q4) {  // as what the codes stand for
+    if (n == 0 || (!keys && !values)) return TMG_OK;
+    CK(launch_kv4_read(kv4_stream(kv->q[layer], stream), kv->q_pos, nullptr, kv->lens[stream],
+                       keys ? kv->q_k : nullptr, values ? kv->q_v : nullptr, kv->kvd, c->d_err,
+                       c->stream),
+       "kv read");
+    if (keys) CK(copy_sync(c, keys, kv->q_k, n * 4, cudaMemcpyDeviceToHost), "kv read");
+    if (values) CK(copy_sync(c, values, kv->q_v, n * 4, cudaMemcpyDeviceToHost), "kv read");
+    return TMG_OK;
+  }
   const size_t off = size_t(stream) * kv->cap * kv->kvd;
   if (keys) CK(copy_sync(c, keys, kv->k[layer] + off, n * 4, cudaMemcpyDeviceToHost), "kv read");
   if (values)
@@ -2014,6 +2211,33 @@ int tmg_forward_seq(tmg_ctx* c, tmg_kv* kv, int32_t stream, const uint32_t* toke
                        c->stream),
        "logits");
   return sync_check(c, "forward_seq");
+}
+
+int tmg_score(tmg_ctx* c, tmg_kv* kv, int32_t stream, const uint32_t* tokens, int64_t T,
+              int32_t n_top, float* logprob, float* entropy, uint32_t* top_ids,
+              float* top_logprobs) {
+  if (!c || !kv || kv->ctx != c || stream < 0 || stream >= kv->M)
+    return fail(c, TMG_ERR_INVALID, "bad argument");
+  if (T <= 0 || !tokens) return fail(c, TMG_ERR_INVALID, "nothing to score");
+  if (!c->finalized) return fail(c, TMG_ERR_INVALID, "weights not finalized");
+  if (c->world > 1) return fail(c, TMG_ERR_INVALID, "tmg_score needs the whole LM head (one GPU)");
+  if (n_top < 0 || n_top > kMaxTopK || n_top > c->V || (n_top > 0 && (!top_ids || !top_logprobs)))
+    return fail(c, TMG_ERR_INVALID,
+                "tmg_score: 0 to 64 alternatives, at most the vocabulary, and room for them");
+  if (!logprob && !entropy && n_top == 0) return fail(c, TMG_ERR_INVALID, "tmg_score: no output");
+  if (kv->lens[stream] + T > kv->cap) return fail(c, TMG_ERR_CAPACITY, "KV cache full");
+  for (int64_t i = 0; i < T; ++i)
+    if (tokens[i] >= uint32_t(c->V)) return fail(c, TMG_ERR_INVALID, "token id out of range");
+  cudaSetDevice(c->device);
+  Scores out;
+  out.n_top = n_top;
+  out.logprob = logprob;
+  out.entropy = entropy;
+  out.top_ids = top_ids;
+  out.top_logprobs = top_logprobs;
+  const int rc = forward_seq(c, kv, stream, tokens, T, true, &out);
+  if (rc) return rc;
+  return sync_check(c, "tmg_score");
 }
 
 int tmg_generate(tmg_ctx* c, tmg_kv* kv, const uint32_t* prompt, int64_t T,
@@ -2174,6 +2398,7 @@ int tmg_trace_decode(tmg_ctx* c, tmg_kv* kv, const uint32_t* tokens, uint64_t* o
                      int32_t* kinds, int32_t max_slots, int32_t* n_slots) {
   if (!c || !kv || kv->ctx != c || !tokens || !out || !kinds || !n_slots)
     return fail(c, TMG_ERR_INVALID, "bad argument");
+  if (kv->q4) return fail(c, TMG_ERR_INVALID, "tmg_trace_decode does not take a 4-bit cache");
   cudaSetDevice(c->device);
   StreamState st;
   int rc = prepare_decode(c, kv, tokens, 2, &st);

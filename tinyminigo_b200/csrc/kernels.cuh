@@ -213,6 +213,13 @@ cudaError_t launch_kv4_append(const Kv4& kv, const float* k, const float* v, int
 // The same rows back to f32 (k or v may be null).
 cudaError_t launch_kv4_read(const Kv4& kv, const int32_t* pos, const int32_t* count, int64_t T,
                             float* k, float* v, int64_t row_ld, int32_t* err, cudaStream_t s);
+// One decode step's qkv rows [M, ld]: q rotated in place, k rotated and
+// quantised with v at pos[m] < cap (the rows of the RoPE tables) of the streams
+// that are not done, lens[m] = the positions that the attention sees.
+cudaError_t launch_kv4_step(const Kv4& kv, float* qkv, int64_t ld, int nq, const StreamState& st,
+                            const float* rope_cos, const float* rope_sin, int cap, int32_t* lens,
+                            cudaStream_t s, bool pdl);
+cudaError_t kv4_prepare();
 struct AttnKv4Args {
   Kv4 kv;
   const float* q = nullptr;  // [M, q_ld]

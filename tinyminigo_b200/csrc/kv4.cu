@@ -156,15 +156,75 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const Rows a) {
   }
 }
 
-template <int D, int U>
-cudaError_t launch_units(const Rows& a, bool append, cudaStream_t s) {
-  const int64_t warps = 2ll * a.kv.M * a.kv.nkv * ((a.T + 256 / D * U - 1) / (256 / D * U));
+// One decode step's rows (q | k | v of every stream, before RoPE): rotates q in
+// place, rotates and quantises k, quantises v, at the stream's position, and
+// gives the attention its length.  A warp a head; the arithmetic of RoPE as
+// everywhere (src/tensor.rs:1026-1037), each product and sum rounded.
+template <int D>
+__global__ void __launch_bounds__(32) kv4_step_kernel(const Kv4 kv, float* qkv, int64_t ld, int nq,
+                                                      StreamState st, const float* rope_cos,
+                                                      const float* rope_sin, int cap,
+                                                      int32_t* lens) {
+  constexpr int G = D < 32 ? D : 32, NG = D / G, E = NG;  // elements a lane: one of each group
+  const int m = blockIdx.y, head = blockIdx.x, lane = threadIdx.x;
+  pdl_trigger();
+  pdl_wait();
+  const int pos = st.pos[m];
+  const bool append = st.done[m] == 0 && pos < cap;
+  if (head == 0 && lane == 0) lens[m] = append ? pos + 1 : min(pos, cap);
+  if (!append && head >= nq) return;
+  float* row = qkv + m * ld + head * D;
+  const bool on = lane < G;
+  float x[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) x[i] = on ? row[i * G + lane] : 0.f;
+  const bool value = head >= nq + kv.nkv;
+  if (!value) {
+    // element e pairs with e + d / 2: another group of the lane, or another lane
+    const int at = min(pos, cap - 1);  // a finished stream may stand behind the last
+    const float* c = rope_cos + int64_t(at) * (D / 2);
+    const float* s = rope_sin + int64_t(at) * (D / 2);
+    float y[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int e = i * G + (lane % G), j = e % (D / 2);
+      const float other = E > 1 ? x[(i + E / 2) % E] : __shfl_xor_sync(0xffffffffu, x[i], D / 2);
+      const float cs = c[j], sn = s[j];
+      y[i] = e < D / 2 ? __fsub_rn(__fmul_rn(x[i], cs), __fmul_rn(other, sn))
+                       : __fadd_rn(__fmul_rn(other, sn), __fmul_rn(x[i], cs));
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = y[i];
+  }
+  if (head < nq) {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (on) row[i * G + lane] = x[i];
+    return;
+  }
+  const int h = value ? head - nq - kv.nkv : head - nq;
+  const int64_t crow = (int64_t(m) * kv.nkv + h) * kv.cap + pos;
+  uint8_t* cb = (value ? kv.vc : kv.kc) + crow * (D / 2);
+  uint32_t* pb = (value ? kv.vp : kv.kp) + crow * NG;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const bool ok = fabsf(x[i]) <= 3.402823466e38f;
+    const float lo = -warp_max(on ? -x[i] : -INFINITY), hi = warp_max(on ? x[i] : -INFINITY);
+    const uint32_t word = kv4_params(lo, hi, __all_sync(0xffffffffu, ok || !on));
+    const uint32_t code = on ? kv4_code(x[i], word) : 0u;
+    const uint32_t next = __shfl_down_sync(0xffffffffu, code, 1);
+    if (on && lane % 2 == 0) cb[(i * G + lane) / 2] = uint8_t(code | (next << 4));
+    if (lane == 0) pb[i] = word;
+  }
+}
+
+template <typename K>
+cudaError_t launch_units(K kern, int U, const Rows& a, cudaStream_t s) {
+  const int64_t rows = 256 / a.kv.d * U;  // a warp's
+  const int64_t warps = 2ll * a.kv.M * a.kv.nkv * ((a.T + rows - 1) / rows);
   const int64_t blocks = (warps + kThreads / 32 - 1) / (kThreads / 32);
   if (blocks > INT32_MAX / (kThreads / 32)) return cudaErrorInvalidValue;
-  if (append)
-    kv4_append_kernel<D, U><<<unsigned(blocks), kThreads, 0, s>>>(a);
-  else
-    kv4_read_kernel<D, U><<<unsigned(blocks), kThreads, 0, s>>>(a);
+  kern<<<unsigned(blocks), kThreads, 0, s>>>(a);
   return cudaGetLastError();
 }
 
@@ -172,9 +232,12 @@ template <int D>
 cudaError_t launch_rows(const Rows& a, bool append, cudaStream_t s) {
   // several units a warp from about two waves of 148 x 64 warps on; 2 to write
   // (4 took 30 us where 2 take 28), 4 to read
-  const int64_t units = 2ll * a.kv.M * a.kv.nkv * ((a.T + 256 / D - 1) / (256 / D));
-  if (units < 18944) return launch_units<D, 1>(a, append, s);
-  return append ? launch_units<D, 2>(a, append, s) : launch_units<D, 4>(a, append, s);
+  const bool many = 2ll * a.kv.M * a.kv.nkv * ((a.T + 256 / D - 1) / (256 / D)) >= 18944;
+  if (append)
+    return many ? launch_units(kv4_append_kernel<D, 2>, 2, a, s)
+                : launch_units(kv4_append_kernel<D, 1>, 1, a, s);
+  return many ? launch_units(kv4_read_kernel<D, 4>, 4, a, s)
+              : launch_units(kv4_read_kernel<D, 1>, 1, a, s);
 }
 
 cudaError_t launch_rows_d(const Rows& a, bool append, cudaStream_t s) {
@@ -188,7 +251,52 @@ cudaError_t launch_rows_d(const Rows& a, bool append, cudaStream_t s) {
   return cudaErrorInvalidValue;
 }
 
+template <int D>
+cudaError_t launch_step(const Kv4& kv, float* qkv, int64_t ld, int nq, const StreamState& st,
+                        const float* rope_cos, const float* rope_sin, int cap, int32_t* lens,
+                        cudaStream_t s, bool pdl) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(nq + 2 * kv.nkv, kv.M);
+  cfg.blockDim = dim3(32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kv4_step_kernel<D>, kv, qkv, ld, nq, st, rope_cos, rope_sin,
+                            cap, lens);
+}
+
+template <int D>
+cudaError_t carveouts() {
+  TMG_CUDA_TRY(set_carveout(kv4_step_kernel<D>));
+  TMG_CUDA_TRY(set_carveout(kv4_append_kernel<D, 1>));
+  TMG_CUDA_TRY(set_carveout(kv4_append_kernel<D, 2>));
+  TMG_CUDA_TRY(set_carveout(kv4_read_kernel<D, 1>));
+  return set_carveout(kv4_read_kernel<D, 4>);
+}
+
 }  // namespace
+
+cudaError_t kv4_prepare() {
+  TMG_CUDA_TRY(carveouts<16>());
+  TMG_CUDA_TRY(carveouts<32>());
+  TMG_CUDA_TRY(carveouts<64>());
+  return carveouts<128>();
+}
+
+cudaError_t launch_kv4_step(const Kv4& kv, float* qkv, int64_t ld, int nq, const StreamState& st,
+                            const float* rope_cos, const float* rope_sin, int cap, int32_t* lens,
+                            cudaStream_t s, bool pdl) {
+  switch (kv.d) {
+    case 16: return launch_step<16>(kv, qkv, ld, nq, st, rope_cos, rope_sin, cap, lens, s, pdl);
+    case 32: return launch_step<32>(kv, qkv, ld, nq, st, rope_cos, rope_sin, cap, lens, s, pdl);
+    case 64: return launch_step<64>(kv, qkv, ld, nq, st, rope_cos, rope_sin, cap, lens, s, pdl);
+    case 128: return launch_step<128>(kv, qkv, ld, nq, st, rope_cos, rope_sin, cap, lens, s, pdl);
+  }
+  return cudaErrorInvalidValue;
+}
 
 cudaError_t launch_kv4_append(const Kv4& kv, const float* k, const float* v, int64_t row_ld,
                               int64_t T, const int32_t* pos, const int32_t* count, int32_t* err,

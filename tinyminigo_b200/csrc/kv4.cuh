@@ -46,6 +46,12 @@ __device__ __forceinline__ uint32_t kv4_params(float lo, float hi, bool ok) {
   return ok ? (m | (s >> 16)) : 0x7fc07fc0u;
 }
 
+// The code of x in a group with parameter word `word`.
+__device__ __forceinline__ uint32_t kv4_code(float x, uint32_t word) {
+  const float s = kv4_step(word);
+  return s > 0.0f ? uint32_t(rint((double(x) - double(kv4_min(word))) / double(s))) : 0u;
+}
+
 // The 8 codes of x in a group with parameter word `word`, lowest first.  The
 // f32 quotient (x - m) / s is off by less than 4e-6 (15 times 2^-22: the
 // difference, the reciprocal and the product), so it decides except next to a
@@ -67,8 +73,7 @@ __device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], uint32_t word
   if (off > 0.5f - 1e-5f || s < 0x1p-126f) {
     codes = 0u;
 #pragma unroll 1
-    for (int j = 7; j >= 0; --j)
-      codes = codes * 16u + uint32_t(rint((double(x[j]) - double(m)) / double(s)));
+    for (int j = 7; j >= 0; --j) codes = codes * 16u + kv4_code(x[j], word);
   }
   return codes;
 }

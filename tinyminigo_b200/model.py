@@ -225,8 +225,9 @@ class Model:
     def last_error(self) -> str:
         return lib().tmg_last_error(self._h).decode()
 
-    def new_cache(self, capacity: int = 4096, n_streams: int = 1) -> "KvCache":
-        return KvCache(self, capacity, n_streams)
+    def new_cache(self, capacity: int = 4096, n_streams: int = 1, bits: int = 32) -> "KvCache":
+        """A cache of f32 rows (bits=32), or of rows in 4 bits (bits=4)."""
+        return KvCache(self, capacity, n_streams, bits)
 
     # --- forwards ---
     def forward_token(self, token, cache: "KvCache", want_logits: bool = True):
@@ -253,6 +254,19 @@ class Model:
                                     _ptr(out) if out is not None else None), self._h,
               "forward_seq")
         return out
+
+    def score(self, tokens, cache: "KvCache", stream: int = 0, top: int = 0) -> "Scores":
+        """forward_seq with every position scored: log probabilities of the
+        tokens that follow, entropies, and the `top` most likely tokens."""
+        t = np.ascontiguousarray(np.asarray(tokens, np.uint32))
+        lp = np.zeros(max(t.size - 1, 0), np.float32)
+        h = np.zeros(t.size, np.float32)
+        ids = np.zeros((t.size, top), np.uint32)
+        tlp = np.zeros((t.size, top), np.float32)
+        check(lib().tmg_score(self._h, cache._h, stream, _ptr(t), t.size, top, _ptr(lp), _ptr(h),
+                              _ptr(ids) if top else None, _ptr(tlp) if top else None), self._h,
+              "score")
+        return Scores(lp, h, ids, tlp)
 
     def prefill(self, tokens, cache: "KvCache", stream: int = 0):
         """Model::prefill: forward_seq that rejects an empty prompt."""
@@ -321,17 +335,34 @@ class Model:
         return out[: n.value * nph * 12].reshape(n.value, nph, 12)
 
 
+@dataclass
+class Scores:
+    """Model.score's result for T tokens."""
+
+    logprobs: np.ndarray      # [T - 1]: of tokens[t + 1] after tokens[:t + 1]
+    entropies: np.ndarray     # [T], nats
+    top_ids: np.ndarray       # [T, top]
+    top_logprobs: np.ndarray  # [T, top]
+
+    def perplexity(self) -> float:
+        return float(np.exp(-np.mean(self.logprobs, dtype=np.float64)))
+
+
 class KvCache:
     """KvCache (src/model.rs:250-332) on the device: per layer and stream an
-    f32 [capacity, n_kv * head_dim] row buffer."""
+    f32 [capacity, n_kv * head_dim] row buffer, or (bits=4) the rows in 4 bits
+    with a bf16 minimum and step for each group of 32 elements."""
 
-    def __init__(self, model: Model, capacity: int, n_streams: int = 1):
+    def __init__(self, model: Model, capacity: int, n_streams: int = 1, bits: int = 32):
+        if bits not in (4, 32):
+            raise ValueError("a cache holds its rows in 32 or 4 bits")
         self.model = model
         self.capacity = capacity
         self.n_streams = n_streams
+        self.bits = bits
         h = ctypes.c_void_p()
-        check(lib().tmg_kv_create(model._h, n_streams, capacity, ctypes.byref(h)), model._h,
-              "kv_create")
+        create = lib().tmg_kv_create if bits == 32 else lib().tmg_kv_create_q4
+        check(create(model._h, n_streams, capacity, ctypes.byref(h)), model._h, "kv_create")
         self._h = h
         if not hasattr(model, "_caches"):
             model._caches = []
@@ -412,14 +443,16 @@ def _gen_cache(model: Model, need: int, n_streams: int) -> KvCache:
 
 
 def generate(model: Model, prompt_tokens, params: GenParams, on_token=None,
-             uniforms=None) -> GenOutput:
+             uniforms=None, cache: KvCache = None) -> GenOutput:
     """generate(): prefill, then the greedy / sampled token loop, all on the
     device; on_token(id) is called for every generated token, in order.
-    `uniforms` overrides the draws of the reference's StdRng(seed)."""
+    `uniforms` overrides the draws of the reference's StdRng(seed); `cache`
+    (one stream, reset first) takes the place of the model's own."""
     p = np.ascontiguousarray(np.asarray(prompt_tokens, np.uint32))
     if p.size == 0:
         raise ValueError("empty prompt")
-    cache = _gen_cache(model, p.size + max(params.max_tokens, 0) + 1, 1)
+    if cache is None:
+        cache = _gen_cache(model, p.size + max(params.max_tokens, 0) + 1, 1)
     maxt = max(params.max_tokens, 0)
     out = np.zeros(max(maxt, 1), np.uint32)
     first = np.zeros(model.config.vocab_size, np.float32)
