@@ -945,7 +945,7 @@ cudaError_t enqueue_forward(tmg_ctx* c, tmg_kv* kv, const StreamState& st, bool 
     B();
     if (kv->q4) {
       TMG_CUDA_TRY(launch_kv4_step(kv->q[l], c->qkv, c->qkv_rows, c->nq, st, kv->rope_cos,
-                                   kv->rope_sin, int(kv->cap), kv->q_lens, c->stream, pdl));
+                                   kv->rope_sin, int(kv->cap), kv->q_lens, c->stream));
       AttnKv4Args Q;
       Q.kv = kv->q[l];
       Q.q = c->qkv;
@@ -959,7 +959,7 @@ cudaError_t enqueue_forward(tmg_ctx* c, tmg_kv* kv, const StreamState& st, bool 
       Q.ws = kv->q_ws;
       Q.err = c->d_err;
       Q.num_sms = c->num_sms;
-      TMG_CUDA_TRY(launch_attn_kv4(Q, c->stream, pdl));
+      TMG_CUDA_TRY(launch_attn_kv4(Q, c->stream));
     } else {
       TMG_CUDA_TRY(launch_attn_decode(T, c->stream, pdl));
     }
@@ -3024,7 +3024,7 @@ int tmg_op_attn_decode_kv4(tmg_ctx* c, const tmg_kv4* view, const float* q, int6
   a.ws = ws;
   a.err = c->d_err;
   a.num_sms = c->num_sms;
-  CK(launch_attn_kv4(a, c->stream, false), "attention");
+  CK(launch_attn_kv4(a, c->stream), "attention");
   return TMG_OK;
 }
 

@@ -162,10 +162,18 @@ struct Plan {
 __device__ __forceinline__ int clamped_len(const AttnKv4Args& a, int m) {
   return min(max(a.lens[m], 0), int(a.max_len));
 }
-// First tile of CTA b of n when `total` tiles are dealt out.
-__device__ __forceinline__ int first_tile(int b, int n, int total) {
-  return int(int64_t(b) * total / n);
-}
+// `total` tiles dealt out to n CTAs (n <= total): the first r take q + 1, the
+// others q.
+struct Deal {
+  int q, r;
+  __device__ __forceinline__ Deal(int total, int n) : q(total / n) { r = total - q * n; }
+  __device__ __forceinline__ int first(int b) const { return b * q + min(b, r); }
+  // the CTA that takes tile T
+  __device__ __forceinline__ int owner(int T) const {
+    const int wide = r * (q + 1);
+    return T < wide ? T / (q + 1) : r + (T - wide) / q;
+  }
+};
 
 // A head group and the tile that a warp has reached in it.
 struct Cursor {
@@ -198,8 +206,8 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
       prefetch_map(&vmap);
     }
   mbar_fence_init();
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();  // the join may start: it reads lens before it waits for this kernel
 
   auto checked_tiles = [&](int m) {
     const int len = a.lens[m];
@@ -250,8 +258,9 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
     __syncthreads();
     const int total = pre[M] * VH, ctas = min(int(gridDim.x), total);
     if (int(blockIdx.x) >= ctas) return;
-    c0 = first_tile(blockIdx.x, ctas, total);
-    c1 = first_tile(blockIdx.x + 1, ctas, total);
+    const Deal deal(total, ctas);
+    c0 = deal.first(blockIdx.x);
+    c1 = deal.first(blockIdx.x + 1);
   } else {  // one head group: its tiles count from 0
     const int m = blockIdx.x / VH, vh = blockIdx.x - m * VH;
     c0 = 0;
@@ -760,7 +769,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
 // CTA each), and zeros for empty streams.  A thread takes 4 columns of one
 // head of every SL-th partial result, so that their loads are in flight
 // together.
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 512;
 template <int D, int NC>
 __global__ void __launch_bounds__(kJoinThreads) attn_kv4_join_kernel(const Plan pl, int grid) {
   using C = Cfg<D, NC>;
@@ -774,55 +783,61 @@ __global__ void __launch_bounds__(kJoinThreads) attn_kv4_join_kernel(const Plan 
   const int VH = pl.VH, m = blockIdx.x / VH, vh = blockIdx.x - m * VH, tid = threadIdx.x;
   const int warp = tid >> 5, lane = tid & 31;
   pdl_trigger();
-  pdl_wait();
+  // everything but the partial results may be read before the main kernel ends
   auto tiles = [&](int i) { return (clamped_len(a, i) + C::TK - 1) / C::TK; };
   int before = 0, total = 0;
+#pragma unroll 1
   for (int i = tid; i < a.kv.M; i += kJoinThreads) {
     const int n = tiles(i);
     total += n;
     if (i < m) before += n;
   }
+  const int nt = tiles(m);
   before = __reduce_add_sync(0xffffffffu, before);
   total = __reduce_add_sync(0xffffffffu, total);
   if (lane == 0) sums[0][warp] = before, sums[1][warp] = total;
-  const int nt = tiles(m);
   __syncthreads();
-  before = total = 0;
-#pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) before += sums[0][w], total += sums[1][w];
+  constexpr int kW = kJoinThreads / 32;
+  before = __reduce_add_sync(0xffffffffu, lane < kW ? sums[0][lane % kW] : 0);
+  total = __reduce_add_sync(0xffffffffu, lane < kW ? sums[1][lane % kW] : 0) * VH;
   const int per = a.nq / a.kv.nkv, g0 = (vh & ((1 << pl.gsh) - 1)) * pl.gh;
   const int heads = min(pl.gh, per - g0);
   float* out = a.out + int64_t(m) * a.out_ld + int64_t((vh >> pl.gsh) * per + g0) * D;
+  int b0 = 0, nb = 1, first = 0;
+  if (nt > 0) {
+    const int s0 = before * VH + vh * nt;
+    const Deal deal(total, min(grid, total));
+    b0 = deal.owner(s0);
+    nb = deal.owner(s0 + nt - 1) - b0 + 1;
+    // only the first of the CTAs can have begun before this head group
+    first = s0 <= deal.first(b0) ? 0 : 1;
+  }
+  pdl_wait();
   if (nt == 0) {
+#pragma unroll 1
     for (int i = tid; i < heads * D; i += kJoinThreads) out[i] = 0.f;
     return;
   }
-  total *= VH;
-  const int s0 = before * VH + vh * nt, s1 = s0 + nt;
-  grid = min(grid, total);  // every CTA that has a run has a tile
-  // the CTA whose run holds tile T
-  auto owner = [&](int T) { return int((int64_t(T + 1) * grid - 1) / total); };
-  const int b0 = owner(s0), nb = owner(s1 - 1) - b0 + 1;
   if (nb == 1) return;
-  // only the first of the CTAs can have begun before this head group
-  const int first = s0 <= first_tile(b0, grid, total) ? 0 : 1;
   auto slot = [&](int i) {
     return pl.part + (int64_t(b0 + i) * 2 + (i == 0 ? first : 0)) * C::SLOT;
   };
-  for (int h = warp; h < heads; h += kJoinThreads / 32) {
+#pragma unroll 1
+  for (int h = warp; h < heads; h += kW) {
     float r = -INFINITY, ls = 0.f;
+#pragma unroll 1
     for (int i = lane; i < nb; i += 32) {
-      const float v = __ldcg(slot(i) + HB * D + h);
+      const float v = __ldcg(slot(i) + HB * D + h), l = __ldcg(slot(i) + HB * D + HB + h);
       fac[i * HB + h] = v;
-      r = fmaxf(r, v);
+      // (the sum so far moves with the reference point)
+      const float n = fmaxf(r, v);
+      ls = fmaf(ls, ex2_approx(r - n), l * ex2_approx(v - n));
+      r = n;
     }
-    r = warp_max(r);
-    for (int i = lane; i < nb; i += 32) {
-      const float f = ex2_approx(fac[i * HB + h] - r);
-      fac[i * HB + h] = f;
-      ls = fmaf(__ldcg(slot(i) + HB * D + HB + h), f, ls);
-    }
-    ls = warp_sum(ls);
+    const float top = warp_max(r);
+    ls = warp_sum(lane < nb ? ls * ex2_approx(r - top) : 0.f);
+#pragma unroll 1
+    for (int i = lane; i < nb; i += 32) fac[i * HB + h] = ex2_approx(fac[i * HB + h] - top);
     if (lane == 0) lsum[h] = ls;
   }
   __syncthreads();
@@ -889,7 +904,7 @@ bool code_map(CUtensorMap* map, const uint8_t* base, const Kv4& kv, int rows) {
 }
 
 template <typename K, typename... A>
-cudaError_t launch(K kern, int grid, int threads, int smem, cudaStream_t s, bool pdl, A... args) {
+cudaError_t launch(K kern, int grid, int threads, int smem, cudaStream_t s, A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
@@ -899,7 +914,7 @@ cudaError_t launch(K kern, int grid, int threads, int smem, cudaStream_t s, bool
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
@@ -908,7 +923,7 @@ cudaError_t launch(K kern, int grid, int threads, int smem, cudaStream_t s, bool
 int head_groups(int per) { return (per + 7) / 8; }
 
 template <int D, int NC>
-cudaError_t run(const AttnKv4Args& a, cudaStream_t s, bool pdl) {
+cudaError_t run(const AttnKv4Args& a, cudaStream_t s) {
   using C = Cfg<D, NC>;
   Plan pl;
   const int per = a.nq / a.kv.nkv;
@@ -924,10 +939,9 @@ cudaError_t run(const AttnKv4Args& a, cudaStream_t s, bool pdl) {
   const int64_t groups = int64_t(a.kv.M) * pl.VH;
   pl.split = a.max_len > 16 * C::TK;
   const int grid = pl.split ? a.num_sms : int(groups);
-  TMG_CUDA_TRY(launch(attn_kv4_kernel<D, NC>, grid, C::W * 32, C::SMEM, s, pdl, km, vm, pl));
+  TMG_CUDA_TRY(launch(attn_kv4_kernel<D, NC>, grid, C::W * 32, C::SMEM, s, km, vm, pl));
   if (!pl.split) return cudaSuccess;
-  return launch(attn_kv4_join_kernel<D, NC>, int(groups), kJoinThreads, grid * C::HB * 4, s, true,
-                pl, grid);
+  return launch(attn_kv4_join_kernel<D, NC>, int(groups), kJoinThreads, grid * C::HB * 4, s, pl, grid);
 }
 
 template <int D, int NC>
@@ -959,17 +973,17 @@ size_t attn_kv4_ws(const Kv4& kv, int nq, int num_sms) {
   return size_t(num_sms) * 2 * (4 * nc) * (kv.d + 2) * 4;  // two of Cfg's SLOT a CTA
 }
 
-cudaError_t launch_attn_kv4(const AttnKv4Args& a, cudaStream_t s, bool pdl) {
+cudaError_t launch_attn_kv4(const AttnKv4Args& a, cudaStream_t s) {
   const int nc = column_tiles(a.nq / a.kv.nkv);
   switch (a.kv.d * 10 + nc) {
-    case 161: return run<16, 1>(a, s, pdl);
-    case 162: return run<16, 2>(a, s, pdl);
-    case 321: return run<32, 1>(a, s, pdl);
-    case 322: return run<32, 2>(a, s, pdl);
-    case 641: return run<64, 1>(a, s, pdl);
-    case 642: return run<64, 2>(a, s, pdl);
-    case 1281: return run<128, 1>(a, s, pdl);
-    case 1282: return run<128, 2>(a, s, pdl);
+    case 161: return run<16, 1>(a, s);
+    case 162: return run<16, 2>(a, s);
+    case 321: return run<32, 1>(a, s);
+    case 322: return run<32, 2>(a, s);
+    case 641: return run<64, 1>(a, s);
+    case 642: return run<64, 2>(a, s);
+    case 1281: return run<128, 1>(a, s);
+    case 1282: return run<128, 2>(a, s);
   }
   return cudaErrorInvalidValue;
 }

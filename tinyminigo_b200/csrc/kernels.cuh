@@ -188,7 +188,8 @@ int attn_decode_noalloc(int device, int num_sms, cudaStream_t s, const float* q,
                         float* out, std::string* why);
 
 // ---------------------------------------------------------------------------
-// The 4-bit KV cache (kv4.cuh: layout and arithmetic).
+// The 4-bit KV cache (kv4.cuh: layout and arithmetic).  These launches are
+// programmatic (PDL): every kernel waits before it touches memory.
 // ---------------------------------------------------------------------------
 // Values of the device error word (1: NaN logits, 2: a bounded wait gave up).
 constexpr int kErrPosition = 3;  // a row's position lies outside the cache
@@ -218,7 +219,7 @@ cudaError_t launch_kv4_read(const Kv4& kv, const int32_t* pos, const int32_t* co
 // that are not done, lens[m] = the positions that the attention sees.
 cudaError_t launch_kv4_step(const Kv4& kv, float* qkv, int64_t ld, int nq, const StreamState& st,
                             const float* rope_cos, const float* rope_sin, int cap, int32_t* lens,
-                            cudaStream_t s, bool pdl);
+                            cudaStream_t s);
 cudaError_t kv4_prepare();
 struct AttnKv4Args {
   Kv4 kv;
@@ -234,7 +235,7 @@ struct AttnKv4Args {
   int32_t* err = nullptr;
   int num_sms = 148;
 };
-cudaError_t launch_attn_kv4(const AttnKv4Args& a, cudaStream_t s, bool pdl);
+cudaError_t launch_attn_kv4(const AttnKv4Args& a, cudaStream_t s);
 cudaError_t attn_kv4_prepare();
 // Bytes of workspace that launch_attn_kv4 needs.
 size_t attn_kv4_ws(const Kv4& kv, int nq, int num_sms);

@@ -65,6 +65,8 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const Rows a) {
   constexpr int G = D < 32 ? D : 32, LG = G / 8;  // lanes a group
   Work w;
   const int lane = threadIdx.x & 31;
+  pdl_trigger();
+  pdl_wait();
   if (!warp_work<D, U>(a, &w)) return;
   const int64_t n = row_count(a, w.m), p0 = a.pos[w.m];
   const float* in = (w.value ? a.v_in : a.k_in) + int64_t(w.m) * a.T * a.ld + w.h * D;
@@ -119,6 +121,8 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const Rows a) {
   constexpr int G = D < 32 ? D : 32;
   Work w;
   const int lane = threadIdx.x & 31;
+  pdl_trigger();
+  pdl_wait();
   if (!warp_work<D, U>(a, &w)) return;
   float* out = w.value ? a.v_out : a.k_out;
   if (out == nullptr) return;
@@ -224,8 +228,16 @@ cudaError_t launch_units(K kern, int U, const Rows& a, cudaStream_t s) {
   const int64_t warps = 2ll * a.kv.M * a.kv.nkv * ((a.T + rows - 1) / rows);
   const int64_t blocks = (warps + kThreads / 32 - 1) / (kThreads / 32);
   if (blocks > INT32_MAX / (kThreads / 32)) return cudaErrorInvalidValue;
-  kern<<<unsigned(blocks), kThreads, 0, s>>>(a);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(blocks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
 template <int D>
@@ -254,7 +266,7 @@ cudaError_t launch_rows_d(const Rows& a, bool append, cudaStream_t s) {
 template <int D>
 cudaError_t launch_step(const Kv4& kv, float* qkv, int64_t ld, int nq, const StreamState& st,
                         const float* rope_cos, const float* rope_sin, int cap, int32_t* lens,
-                        cudaStream_t s, bool pdl) {
+                        cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(nq + 2 * kv.nkv, kv.M);
   cfg.blockDim = dim3(32);
@@ -263,7 +275,7 @@ cudaError_t launch_step(const Kv4& kv, float* qkv, int64_t ld, int nq, const Str
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kv4_step_kernel<D>, kv, qkv, ld, nq, st, rope_cos, rope_sin,
                             cap, lens);
 }
@@ -288,12 +300,12 @@ cudaError_t kv4_prepare() {
 
 cudaError_t launch_kv4_step(const Kv4& kv, float* qkv, int64_t ld, int nq, const StreamState& st,
                             const float* rope_cos, const float* rope_sin, int cap, int32_t* lens,
-                            cudaStream_t s, bool pdl) {
+                            cudaStream_t s) {
   switch (kv.d) {
-    case 16: return launch_step<16>(kv, qkv, ld, nq, st, rope_cos, rope_sin, cap, lens, s, pdl);
-    case 32: return launch_step<32>(kv, qkv, ld, nq, st, rope_cos, rope_sin, cap, lens, s, pdl);
-    case 64: return launch_step<64>(kv, qkv, ld, nq, st, rope_cos, rope_sin, cap, lens, s, pdl);
-    case 128: return launch_step<128>(kv, qkv, ld, nq, st, rope_cos, rope_sin, cap, lens, s, pdl);
+    case 16: return launch_step<16>(kv, qkv, ld, nq, st, rope_cos, rope_sin, cap, lens, s);
+    case 32: return launch_step<32>(kv, qkv, ld, nq, st, rope_cos, rope_sin, cap, lens, s);
+    case 64: return launch_step<64>(kv, qkv, ld, nq, st, rope_cos, rope_sin, cap, lens, s);
+    case 128: return launch_step<128>(kv, qkv, ld, nq, st, rope_cos, rope_sin, cap, lens, s);
   }
   return cudaErrorInvalidValue;
 }
