@@ -151,6 +151,33 @@ __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
   }
   return r * (D / 2) + c * 16;
 }
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
+
 // The tiles of all streams, in order of (stream, head group, tile).
 struct Plan {
   AttnKv4Args a;
@@ -485,10 +512,6 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
     const int seg_first = cur.m * VH + cur.vh;
     start(q);
     bool whole = cur.tile == 0;  // the head group began in this warp
-    // the row that this lane addresses in a ldmatrix of 16 positions and two
-    // groups (D >= 64; of 32 positions for D = 32): matrices in order (8 rows,
-    // next 8 rows) x groups
-    const int lrow = D == 32 ? lane : lane & 15, lgrp = D == 32 ? 0 : lane >> 4;
     int st = 0;
     uint32_t phase = 0;
     for (int T = w0; T < w1; ++T) {
@@ -501,47 +524,51 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
       const int valid = len - cur.tile * TK;  // positions of the tile in the row
 
       // scores of positions 16 b + 8 i + g, x[][2 b + i]
-      [[maybe_unused]] uint32_t kw[4];
       float x[NC][2 * KB];
 #pragma unroll
       for (int b = 0; b < KB; ++b) {
-        uint32_t p0[NG], p1[NG], w[NG][2];  // parameters and code words of the two rows
-        lds_words<NG>(base + 2 * C::CODE + (16 * b + g) * NG * 4, p0);
-        lds_words<NG>(base + 2 * C::CODE + (16 * b + 8 + g) * NG * 4, p1);
-        if constexpr (D == 16) {  // two bytes: one to each half
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            w[0][i] = __byte_perm(lds32(base + (16 * b + 8 * i + g) * 8 + (t >> 1) * 4), 0u,
-                                  t & 1 ? 0x4342u : 0x4140u);
-        } else if constexpr (D == 32) {
-          if (b % 2 == 0) ldsm(base + (16 * b + lrow) * 16, kw);
-          w[0][0] = kw[b % 2 * 2], w[0][1] = kw[b % 2 * 2 + 1];
-        } else {
-#pragma unroll
-          for (int j = 0; j < NG; j += 2) {
-            uint32_t v[4];
-            ldsm(base + chunk_off<D>(16 * b + lrow, j + lgrp), v);
-            w[j][0] = v[0], w[j][1] = v[1], w[j + 1][0] = v[2], w[j + 1][1] = v[3];
-          }
-        }
 #pragma unroll
         for (int k = 0; k < NC; ++k) x[k][2 * b] = x[k][2 * b + 1] = 0.f;
+      }
+#pragma unroll
+      for (int b2 = 0; b2 < KB; b2 += 2) {
+        uint32_t par[4][NG];  // parameters of the rows 16 b2 + 8 i + g
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          lds_words<NG>(base + 2 * C::CODE + (16 * b2 + 8 * i + g) * NG * 4, par[i]);
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-          const uint32_t u = w[j][0], v = w[j][1];
-          const float s0 = kv4_step(p0[j]), m0 = kv4_min(p0[j]);
-          const float s1 = kv4_step(p1[j]), m1 = kv4_min(p1[j]);
+          uint32_t w[4];  // code words of those rows
+          if constexpr (D == 16) {  // two bytes: one to each half
 #pragma unroll
-          for (int k = 0; k < NC; ++k) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
-            // codes as f16 numbers below 1: c * 2^-24, 16 c * 2^-24
-            mma_f16(c, u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
-                    qb[k][j][0], qb[k][j][1]);
-            if constexpr (D > 16)
-              mma_f16(c, (u >> 8) & 0x000f000fu, (v >> 8) & 0x000f000fu, (u >> 8) & 0x00f000f0u,
-                      (v >> 8) & 0x00f000f0u, qb[k][j][2], qb[k][j][3]);
-            x[k][2 * b] = fmaf(s0, c[0] + c[1], fmaf(m0, qs[k][j], x[k][2 * b]));
-            x[k][2 * b + 1] = fmaf(s1, c[2] + c[3], fmaf(m1, qs[k][j], x[k][2 * b + 1]));
+            for (int i = 0; i < 4; ++i)
+              w[i] = __byte_perm(lds32(base + (16 * b2 + 8 * i + g) * 8 + (t >> 1) * 4), 0u,
+                                 t & 1 ? 0x4342u : 0x4140u);
+          } else {
+            ldsm(base + chunk_off<D>(16 * b2 + lane, j), w);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const int b = b2 + i / 2;
+            const uint32_t u = w[i], v = w[i + 1];
+            const float s0 = kv4_step(par[i][j]), m0 = kv4_min(par[i][j]);
+            const float s1 = kv4_step(par[i + 1][j]), m1 = kv4_min(par[i + 1][j]);
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+              float c[4] = {0.f, 0.f, 0.f, 0.f};
+              // codes as f16 numbers below 1: c * 2^-24, 16 c * 2^-24
+              mma_f16(c, u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
+                      qb[k][j][0], qb[k][j][1]);
+              if constexpr (D > 16)
+                mma_f16(c, (u >> 8) & 0x000f000fu, (v >> 8) & 0x000f000fu,
+                        (u >> 8) & 0x00f000f0u, (v >> 8) & 0x00f000f0u, qb[k][j][2], qb[k][j][3]);
+              const float2 v2 =
+                  fma2(make_float2(s0, s1), make_float2(c[0] + c[1], c[2] + c[3]),
+                       fma2(make_float2(m0, m1), twice(qs[k][j]),
+                            make_float2(x[k][2 * b], x[k][2 * b + 1])));
+              x[k][2 * b] = v2.x;
+              x[k][2 * b + 1] = v2.y;
+            }
           }
         }
       }
@@ -617,7 +644,6 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
           p[k][i] = ex2_approx(fmaf(x[k][i], cq[k], -ref[k]));
           l[k] += p[k][i];
         }
-      [[maybe_unused]] uint32_t vw[KB][4];
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         uint32_t pb[NC][2 * KB];
@@ -631,12 +657,12 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
           }
         }
         float c[NC][2][4] = {};
+        uint32_t w[4];
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
           // the codes of 4 dims of positions 16 b + 2 t, + 1 (u) and + 8, + 9 (v)
           uint32_t u, v;
           if constexpr (D == 16) {  // byte g of the rows
-            uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               w[i] = lds32(base + C::CODE + (16 * b + 8 * (i >> 1) + 2 * t + (i & 1)) * 8 +
@@ -644,12 +670,9 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
             const uint32_t sel = (g & 3) | (4 + (g & 3)) << 8;
             u = __byte_perm(w[0], w[1], sel);
             v = __byte_perm(w[2], w[3], sel);
-          } else if constexpr (D == 32) {
-            if (b % 2 == 0) ldsm_t(base + C::CODE + (16 * b + lrow) * 16, vw[0]);
-            u = vw[0][b % 2 * 2], v = vw[0][b % 2 * 2 + 1];
           } else {
-            if (j % 2 == 0) ldsm_t(base + C::CODE + chunk_off<D>(16 * b + lrow, j + lgrp), vw[b]);
-            u = vw[b][j % 2 * 2], v = vw[b][j % 2 * 2 + 1];
+            if (b % 2 == 0) ldsm_t(base + C::CODE + chunk_off<D>(16 * b + lane, j), w);
+            u = w[b % 2 * 2], v = w[b % 2 * 2 + 1];
           }
           const uint32_t a0 = centred_lo(u), a1 = centred_hi(u);
           const uint32_t a2 = centred_lo(v), a3 = centred_hi(v);
