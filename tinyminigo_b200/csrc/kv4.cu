@@ -8,6 +8,8 @@
 // parameters (32 or 64) that are whole sectors of the cache.  The f32 side
 // goes 16 bytes a lane, a warp's 512 in one piece; 4 units a warp, their loads
 // in flight together, once there are enough rows to fill the GPU so.
+#include <algorithm>
+
 #include "kv4.cuh"
 
 namespace tmg {
@@ -25,92 +27,100 @@ struct Rows {
   int32_t* err;
 };
 
-// A warp's work: U units from row t0 of one head of one stream, keys or values.
+// Blocks: x the head (keys, then values; all heads of a row at once, since
+// they are neighbours in memory), y a stretch of rows, z the stream.  A warp's
+// rows w.t0 .. w.t0 + 256 / d * U - 1 of that head.
 struct Work {
   bool value;
-  int h, m;
-  int64_t t0;
+  int h;
+  int64_t n;     // rows of the stream that are no padding
+  int64_t p0;    // position of row 0
+  int64_t row0;  // cache row of position 0
 };
-template <int D, int U>
-__device__ __forceinline__ bool warp_work(const Rows& a, Work* o) {
-  constexpr int R = 256 / D * U;  // rows
-  const unsigned nt = unsigned((a.T + R - 1) / R), n = 2u * a.kv.nkv;
-  unsigned w = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
-  const unsigned c = w % n;
-  w /= n;
-  o->value = int(c) >= a.kv.nkv;
-  o->h = o->value ? int(c) - a.kv.nkv : int(c);
-  o->t0 = int64_t(w % nt) * R;
-  o->m = int(w / nt);
-  return o->m < a.kv.M;
+__device__ __forceinline__ Work block_work(const Rows& a) {
+  Work w;
+  const int m = blockIdx.z;
+  w.value = int(blockIdx.x) >= a.kv.nkv;
+  w.h = int(blockIdx.x) - (w.value ? a.kv.nkv : 0);
+  w.n = a.count ? min(a.T, int64_t(max(a.count[m], 0))) : a.T;
+  w.p0 = a.pos[m];
+  w.row0 = (int64_t(m) * a.kv.nkv + w.h) * a.kv.cap;
+  return w;
+}
+// Whether position p lies in the cache (reported if not).
+__device__ __forceinline__ bool in_cache(const Rows& a, int64_t p) {
+  if (p >= 0 && p < a.kv.cap) return true;
+  if (a.err) atomicCAS(a.err, 0, kErrPosition);
+  return false;
 }
 
-// Rows of stream m that are no padding, and the first one's position.
-__device__ __forceinline__ int64_t row_count(const Rows& a, int m) {
-  return a.count ? min(a.T, int64_t(max(a.count[m], 0))) : a.T;
+// The smaller / larger of two, NaN if either is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
 }
-// The cache row of position p, or -1 (reported) outside the cache.
-__device__ __forceinline__ int64_t cache_row(const Rows& a, const Work& w, int64_t p) {
-  if (p < 0 || p >= a.kv.cap) {
-    if (a.err) atomicCAS(a.err, 0, kErrPosition);
-    return -1;
-  }
-  return (int64_t(w.m) * a.kv.nkv + w.h) * a.kv.cap + p;
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
 }
 
-// 8 elements a lane: a group's arithmetic (a division among it) is repeated
-// by 4 lanes and not by 8.
+// 8 elements a lane: a group's arithmetic is repeated by 4 lanes and not by 8.
 template <int D, int U>
 __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const Rows a) {
   constexpr int G = D < 32 ? D : 32, LG = G / 8;  // lanes a group
-  Work w;
-  const int lane = threadIdx.x & 31;
+  constexpr int R = 256 / D;                      // rows a unit
   pdl_trigger();
   pdl_wait();
-  if (!warp_work<D, U>(a, &w)) return;
-  const int64_t n = row_count(a, w.m), p0 = a.pos[w.m];
-  const float* in = (w.value ? a.v_in : a.k_in) + int64_t(w.m) * a.T * a.ld + w.h * D;
-  const int t0 = lane * 8 / D, e = lane * 8 % D;  // the lane's row of a unit, and column
-  float4 v[U][2];
+  const Work w = block_work(a);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int e = lane * 8 % D;  // the lane's column; its row of a unit: lane * 8 / D
+  const float* in = (w.value ? a.v_in : a.k_in) + int64_t(blockIdx.z) * a.T * a.ld + w.h * D + e;
+  uint8_t* cb = (w.value ? a.kv.vc : a.kv.kc) + e / 2;
+  uint32_t* pb = (w.value ? a.kv.vp : a.kv.kp) + e / G;
+  constexpr int kBlock = kThreads / 32 * U * R;  // rows a block and round
+#pragma unroll 1
+  for (int64_t tb = int64_t(blockIdx.y) * kBlock; tb < w.n; tb += int64_t(gridDim.y) * kBlock) {
+    const int64_t t0 = tb + warp * (U * R) + lane * 8 / D;
+    const float* src = in + t0 * a.ld;
+    float4 v[U][2];
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int64_t t = w.t0 + i * (256 / D) + t0;
-    v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (t < n) {
-      const float4* p = reinterpret_cast<const float4*>(in + t * a.ld + e);
-      v[i][0] = __ldg(p);
-      v[i][1] = __ldg(p + 1);
+    for (int i = 0; i < U; ++i) {
+      v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (t0 + i * R < w.n) {
+        v[i][0] = __ldg(reinterpret_cast<const float4*>(src));
+        v[i][1] = __ldg(reinterpret_cast<const float4*>(src) + 1);
+      }
+      src += R * a.ld;
     }
-  }
-  uint8_t* cb = w.value ? a.kv.vc : a.kv.kc;
-  uint32_t* pb = w.value ? a.kv.vp : a.kv.kp;
+    const int64_t row = w.row0 + w.p0 + t0;
+    uint8_t* cd = cb + row * (D / 2);
+    uint32_t* pd = pb + row * (D / G);
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const float x[8] = {v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w,
-                        v[i][1].x, v[i][1].y, v[i][1].z, v[i][1].w};
-    float lo = x[0], hi = x[0];
-    bool ok = true;
+    for (int i = 0; i < U; ++i) {
+      const float x[8] = {v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w,
+                          v[i][1].x, v[i][1].y, v[i][1].z, v[i][1].w};
+      float lo = x[0], hi = x[0];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      lo = fminf(lo, x[j]);
-      hi = fmaxf(hi, x[j]);
-      ok = ok && fabsf(x[j]) <= 3.402823466e38f;
+      for (int j = 1; j < 8; ++j) {
+        lo = min_nan(lo, x[j]);
+        hi = max_nan(hi, x[j]);
+      }
+#pragma unroll
+      for (int o = 1; o < LG; o <<= 1) {
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      }
+      const uint32_t word =
+          kv4_params(lo, hi, lo >= -3.402823466e38f && hi <= 3.402823466e38f);
+      const uint32_t codes = kv4_codes(x, word);
+      const int64_t t = t0 + i * R;
+      if (t < w.n && in_cache(a, w.p0 + t)) {
+        *reinterpret_cast<uint32_t*>(cd + i * R * (D / 2)) = codes;
+        if (lane % LG == 0) pd[i * R * (D / G)] = word;
+      }
     }
-    // the group's extremes over its lanes; +inf above stands for a value that
-    // is not finite
-    hi = ok ? hi : INFINITY;
-#pragma unroll
-    for (int o = 1; o < LG; o <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    const uint32_t word = kv4_params(lo, hi, hi < INFINITY);
-    const uint32_t codes = kv4_codes(x, word);
-    const int64_t t = w.t0 + i * (256 / D) + t0;
-    const int64_t row = t < n ? cache_row(a, w, p0 + t) : -1;
-    if (row < 0) continue;
-    *reinterpret_cast<uint32_t*>(cb + row * (D / 2) + e / 2) = codes;
-    if (lane % LG == 0) pb[row * (D / G) + e / G] = word;
   }
 }
 
@@ -118,45 +128,51 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const Rows a) {
 // is in row (128 i + 4 lane) / d of the warp's, column (128 i + 4 lane) % d.
 template <int D, int U>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const Rows a) {
-  constexpr int G = D < 32 ? D : 32;
-  Work w;
-  const int lane = threadIdx.x & 31;
+  constexpr int G = D < 32 ? D : 32, R = 256 / D;
   pdl_trigger();
   pdl_wait();
-  if (!warp_work<D, U>(a, &w)) return;
+  const Work w = block_work(a);
   float* out = w.value ? a.v_out : a.k_out;
   if (out == nullptr) return;
-  const int64_t n = row_count(a, w.m), p0 = a.pos[w.m];
-  const uint8_t* cb = w.value ? a.kv.vc : a.kv.kc;
-  const uint32_t* pb = w.value ? a.kv.vp : a.kv.kp;
-  // codes 8 a lane, as whole sectors
-  uint32_t c[U], word[U];
-  bool on[U];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int e = lane * 8 % D;
+  const uint8_t* cb = (w.value ? a.kv.vc : a.kv.kc) + e / 2;
+  const uint32_t* pb = (w.value ? a.kv.vp : a.kv.kp) + e / G;
+  out += int64_t(blockIdx.z) * a.T * a.ld + w.h * D;
+  constexpr int kBlock = kThreads / 32 * U * R;
+#pragma unroll 1
+  for (int64_t tb = int64_t(blockIdx.y) * kBlock; tb < w.n; tb += int64_t(gridDim.y) * kBlock) {
+    const int64_t tw = tb + warp * (U * R), t0 = tw + lane * 8 / D;
+    const int64_t row = w.row0 + w.p0 + t0;
+    const uint8_t* cs = cb + row * (D / 2);
+    const uint32_t* ps = pb + row * (D / G);
+    // codes 8 a lane, as whole sectors
+    uint32_t c[U], word[U];
+    bool on[U];
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int e = i * 256 + lane * 8;
-    const int64_t t = w.t0 + e / D;
-    const int64_t row = t < n ? cache_row(a, w, p0 + t) : -1;
-    on[i] = row >= 0;
-    c[i] = word[i] = 0;
-    if (on[i]) {
-      c[i] = __ldg(reinterpret_cast<const uint32_t*>(cb + row * (D / 2) + e % D / 2));
-      word[i] = __ldg(pb + row * (D / G) + e % D / G);
+    for (int i = 0; i < U; ++i) {
+      const int64_t t = t0 + i * R;
+      on[i] = t < w.n && in_cache(a, w.p0 + t);
+      c[i] = word[i] = 0;
+      if (on[i]) {
+        c[i] = __ldg(reinterpret_cast<const uint32_t*>(cs + i * R * (D / 2)));
+        word[i] = __ldg(ps + i * R * (D / G));
+      }
     }
-  }
-  out += int64_t(w.m) * a.T * a.ld + w.h * D;
 #pragma unroll
-  for (int i = 0; i < 2 * U; ++i) {
-    // 4 of the 8 codes that lane 16 (i % 2) + lane / 2 has loaded
-    const int src = 16 * (i % 2) + lane / 2;
-    const uint32_t cc = __shfl_sync(0xffffffffu, c[i / 2], src) >> (16 * (lane & 1));
-    const uint32_t ww = __shfl_sync(0xffffffffu, word[i / 2], src);
-    if (!__shfl_sync(0xffffffffu, int(on[i / 2]), src)) continue;
-    const float m = kv4_min(ww), s = kv4_step(ww);
-    const int e = i * 128 + lane * 4;
-    __stcs(reinterpret_cast<float4*>(out + (w.t0 + e / D) * a.ld + e % D),
-           make_float4(fmaf(float(cc & 15u), s, m), fmaf(float((cc >> 4) & 15u), s, m),
-                       fmaf(float((cc >> 8) & 15u), s, m), fmaf(float((cc >> 12) & 15u), s, m)));
+    for (int i = 0; i < 2 * U; ++i) {
+      // 4 of the 8 codes that lane 16 (i % 2) + lane / 2 has loaded
+      const int from = 16 * (i % 2) + lane / 2;
+      const uint32_t cc = __shfl_sync(0xffffffffu, c[i / 2], from) >> (16 * (lane & 1));
+      const uint32_t ww = __shfl_sync(0xffffffffu, word[i / 2], from);
+      const bool store = __shfl_sync(0xffffffffu, int(on[i / 2]), from);
+      const float m = kv4_min(ww), s = kv4_step(ww);
+      const int q = i * 128 + lane * 4;
+      if (store)
+        __stcs(reinterpret_cast<float4*>(out + (tw + q / D) * a.ld + q % D),
+               make_float4(fmaf(float(cc & 15u), s, m), fmaf(float((cc >> 4) & 15u), s, m),
+                           fmaf(float((cc >> 8) & 15u), s, m), fmaf(float((cc >> 12) & 15u), s, m)));
+    }
   }
 }
 
@@ -224,12 +240,9 @@ __global__ void __launch_bounds__(32) kv4_step_kernel(const Kv4 kv, float* qkv, 
 
 template <typename K>
 cudaError_t launch_units(K kern, int U, const Rows& a, cudaStream_t s) {
-  const int64_t rows = 256 / a.kv.d * U;  // a warp's
-  const int64_t warps = 2ll * a.kv.M * a.kv.nkv * ((a.T + rows - 1) / rows);
-  const int64_t blocks = (warps + kThreads / 32 - 1) / (kThreads / 32);
-  if (blocks > INT32_MAX / (kThreads / 32)) return cudaErrorInvalidValue;
+  const int64_t rows = int64_t(kThreads / 32) * U * 256 / a.kv.d;  // a block's
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(blocks));
+  cfg.gridDim = dim3(2 * a.kv.nkv, unsigned(std::min<int64_t>((a.T + rows - 1) / rows, 65535)), a.kv.M);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];

@@ -61,15 +61,19 @@ __device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], uint32_t word
   if (!(s > 0.0f)) return 0u;  // a constant group, or one that stands for NaN
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: a sum's low bits are the rounded t
-  uint32_t codes = 0u;
+  // a sum with 1.5 * 2^23 has the rounded t in its low bits, above them
+  // 0x4b400000, which the codes' places take off again
+  constexpr float kMagic = 12582912.0f;
+  uint32_t codes = 0u - 0x4b400000u * 0x11111111u;
+  uint32_t sum = 0u;
   float off = 0.0f;
 #pragma unroll
   for (int j = 7; j >= 0; --j) {
     const float t = (x[j] - m) * inv, r = t + kMagic;
     off = fmaxf(off, fabsf(t - (r - kMagic)));
-    codes = codes * 16u + (__float_as_uint(r) & 15u);
+    sum = sum * 16u + __float_as_uint(r);
   }
+  codes += sum;
   if (off > 0.5f - 1e-5f || s < 0x1p-126f) {
     codes = 0u;
 #pragma unroll 1
