@@ -960,7 +960,12 @@ cudaError_t run(const AttnKv4Args& a, cudaStream_t s) {
   if (C::MAP && (!code_map(&km, a.kv.kc, a.kv, C::TK) || !code_map(&vm, a.kv.vc, a.kv, C::TK)))
     return cudaErrorInvalidValue;
   const int64_t groups = int64_t(a.kv.M) * pl.VH;
-  pl.split = a.max_len > 16 * C::TK;
+  // A CTA a head group, or every CTA an equal run of the tiles and a join: the
+  // join and what prepares it cost about 4 us, so up to 32 tiles a head group
+  // (2 a warp; 64 where the head groups fill the GPU by half) go without.
+  // 2048 positions of 8 heads of 64: 10.2 and 10.6 us; 4096: 14.8 and 10.9; 128
+  // groups of 2048 (heads of 128): 16.4 and 20.5 us.
+  pl.split = groups > a.num_sms || a.max_len > (2 * groups > a.num_sms ? 64 : 32) * C::TK;
   const int grid = pl.split ? a.num_sms : int(groups);
   TMG_CUDA_TRY(launch(attn_kv4_kernel<D, NC>, grid, C::W * 32, C::SMEM, s, km, vm, pl));
   if (!pl.split) return cudaSuccess;

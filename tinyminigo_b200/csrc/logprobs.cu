@@ -82,26 +82,33 @@ struct Row {
   }
 };
 
-// A thread's pass over its chunks: the online state, and the index of the
-// first of its largest elements.
+// A thread's pass over its chunks: the online state, the index of the first of
+// its largest elements, and the second largest value.
 struct Pass {
   Soft s;
   uint32_t idx;
+  float second = -INFINITY;
   template <int U>
   __device__ __forceinline__ void take(const float4 (&v)[U], int c, int shift) {
     float mx = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u)
       mx = fmaxf(mx, fmaxf(fmaxf(v[u].x, v[u].y), fmaxf(v[u].z, v[u].w)));
-    if (mx > s.x) {
+    if (mx > second) {  // a few times a row
+      float best = s.x;
 #pragma unroll
-      for (int u = U - 1; u >= 0; --u) {
+      for (int u = 0; u < U; ++u) {
         const float x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
-        for (int j = 3; j >= 0; --j)
-          if (x[j] == mx) idx = uint32_t(4 * (c + u * kThreads) + j - shift);
+        for (int j = 0; j < 4; ++j) {
+          second = fmaxf(second, fminf(best, x[j]));
+          if (x[j] > best) {
+            best = x[j];
+            idx = uint32_t(4 * (c + u * kThreads) + j - shift);
+          }
+        }
       }
-      move(s, mx);
+      if (best > s.x) move(s, best);
     }
     const float ref = s.x == -INFINITY ? 0.f : s.x;
 #pragma unroll
@@ -147,6 +154,7 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const LogprobsArg
   __shared__ unsigned or_s[kW], and_s[kW];
   __shared__ u64 cand[kCand];
   __shared__ int owner[kMaxTopK + kSlack];
+  __shared__ u64 owner_key[kMaxTopK + kSlack];
   __shared__ int n_owner, n_cand, n_s;
   __shared__ Parts parts;
   cg::cluster_group cluster = cg::this_cluster();
@@ -219,8 +227,11 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const LogprobsArg
 
   // Alternatives.  A thread's largest key is an element; the n_top-th largest of
   // them (or a bound that a few more reach) bounds the slice's n_top-th largest
-  // element from below, and only the threads at or above it can hold an
-  // element that is: their elements are looked at again.
+  // element from below.  The threads at or above it (owners) bring theirs; an
+  // owner has others there only if its second largest value reaches the bound
+  // too, and only such owners' elements are looked at again: by then they may
+  // have left L2 (reading every owner's cost 75 of 250 us for 64 alternatives of
+  // 2047 x 128256).
   int n = 0;
   if (a.n_top) {
     const unsigned any = __reduce_or_sync(0xffffffffu, or_s[lane % kW]);
@@ -241,19 +252,26 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const LogprobsArg
     } else {
       tau = 0ull;
     }
-    if (mine >= tau && mine != 0ull) {
-      const int i = atomicAdd(&n_owner, 1);
-      if (i < kMaxTopK + kSlack) owner[i] = tid;
+    if (mine >= tau && mine != 0ull && order_key(ps.second, 0u) >= tau) {
+      const int w = atomicAdd(&n_owner, 1);  // at most n_top + kSlack
+      if (w < kMaxTopK + kSlack) owner[w] = tid, owner_key[w] = mine;
     }
     __syncthreads();
-    const bool all = n_owner < a.n_top;  // fewer threads with elements than wanted
-    const int owners = all ? min(kThreads, c1 - c0) : min(n_owner, kMaxTopK + kSlack);
+    const int owners = min(n_owner, kMaxTopK + kSlack);
     const int per = (c1 - c0 + kThreads - 1) / kThreads;
     auto collect = [&](u64 t, bool keep) {
       int m = 0;
+      if (mine >= t && mine != 0ull) {
+        ++m;
+        if (keep) {
+          const int at = atomicAdd(&n_cand, 1);
+          if (at < kCand) cand[at] = mine;
+        }
+      }
 #pragma unroll 1
       for (int w = warp; w < owners; w += kW) {
-        const int first = c0 + (all ? w : owner[w]);
+        const int first = c0 + owner[w];
+        const u64 had = owner_key[w];
 #pragma unroll 1
         for (int i = lane; i < per; i += 32) {
           const int c = first + i * kThreads;
@@ -263,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const LogprobsArg
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const u64 k = R.key(x[j], c, j);
-            if (k != 0ull && k >= t) {
+            if (k != 0ull && k >= t && k != had) {
               ++m;
               if (keep) {
                 const int at = atomicAdd(&n_cand, 1);
@@ -375,10 +393,10 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const LogprobsArg
 
 cudaError_t launch_logprobs(const LogprobsArgs& a, cudaStream_t s, int num_sms) {
   if (a.rows == 0) return cudaSuccess;
-  // Few rows: a cluster of CTAs a row, up to two CTAs an SM in all and no
-  // slice below 4 loads a thread.
+  // Few rows: a cluster of CTAs a row, up to the three CTAs that an SM holds
+  // and no slice below 4 loads a thread.
   int slices = 1;
-  while (slices < kMaxSlices && a.rows * slices * 2 <= 2 * num_sms &&
+  while (slices < kMaxSlices && a.rows * slices * 2 <= 3 * num_sms &&
          a.V >= int64_t(slices) * 2 * kThreads * 16)
     slices *= 2;
   cudaLaunchConfig_t cfg = {};
