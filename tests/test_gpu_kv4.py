@@ -245,6 +245,29 @@ def test_large_offsets(ctx):
     assert c.guards_intact()
 
 
+def test_more_rows_than_a_grid_has_blocks(ctx):
+    # 65535 blocks of 32 rows (heads of 128) and some: the blocks go round
+    T, d = 65535 * 32 + 75, 128
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GB free")
+    cap = (T + 3) // 4 * 4
+    c = Cache(1, 1, d, cap)
+    x = torch.randn(T, 2 * d, generator=torch.Generator(device="cuda").manual_seed(3),
+                    device="cuda")
+    out = torch.full((2, T, d), -7.0, device="cuda")
+    pos = torch.zeros(1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    check(lib().tmg_op_kv4_append(ctx, c.ref(), P(x), P(x, 4 * d), 2 * d, T, P(pos), None), ctx)
+    check(lib().tmg_op_kv4_read(ctx, c.ref(), P(pos), None, T, P(out[0]), P(out[1]), d), ctx)
+    check(lib().tmg_sync(ctx), ctx)
+    assert c.guards_intact() and not bool((out == -7.0).any())
+    for at in (0, 65535 * 16, 65535 * 32 - 5, T - 80):
+        part = x[at:at + 80].cpu().numpy()
+        for i in range(2):
+            want = R.values(*R.quantise(part[:, i * d:(i + 1) * d])).astype(np.float32)
+            assert np.array_equal(out[i, at:at + 80].cpu().numpy(), want)
+
+
 # ---------------------------------------------------------------------------
 # Attention
 # ---------------------------------------------------------------------------
@@ -498,6 +521,41 @@ def test_captured_and_replayed(ctx):
         refs, tols = expect(c, q.cpu().numpy().reshape(M, n_q, d), now.cpu().tolist())
         for m in range(M):
             assert np.abs(got[m].cpu().numpy().reshape(n_q, d) - refs[m]).max() <= tols[m]
+    del graph
+
+
+def test_captured_behind_other_work(ctx):
+    # a copy and a kernel of the caller's before the calls, in one graph, and
+    # the lengths read from what that copy brings
+    rng = np.random.default_rng(32)
+    M, n_kv, n_q, d, cap = 2, 2, 8, 128, 4096
+    lens = [4096, 2500]
+    c = filled(rng, M, n_kv, d, cap, lens)
+    src = torch.zeros((M, n_q * d), device="cuda")
+    q = torch.zeros_like(src)
+    now, new = (torch.zeros(M, dtype=torch.int32, device="cuda") for _ in range(2))
+    out = torch.zeros_like(src)
+    ws, n = workspace(ctx, c, n_q)
+    stream = torch.cuda.ExternalStream(lib().tmg_stream(ctx))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        torch.mul(src, 0.5, out=q)
+        now.copy_(new)
+        check(lib().tmg_op_attn_decode_kv4(ctx, c.ref(), P(q), n_q * d, P(now), cap, n_q, P(out),
+                                           n_q * d, P(ws), n), ctx)
+        out.mul_(2.0)
+    for lens in ([4096, 2500], [3, 2222], [0, 2049]):
+        src.copy_(dev(rng.normal(0, 2, tuple(src.shape)).astype(np.float32)))
+        new.copy_(dev(np.asarray(lens, np.int32)))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+            graph.replay()
+        check(lib().tmg_sync(ctx), ctx)
+        refs, tols = expect(c, q.cpu().numpy().reshape(M, n_q, d), lens)
+        for m in range(M):
+            assert np.abs(out[m].cpu().numpy().reshape(n_q, d) / 2 - refs[m]).max() <= tols[m]
     del graph
 
 

@@ -13,11 +13,24 @@
 // 8 s_t): p s in two f16 parts; the codes centred, since the sums of c and
 // of m alone are hundreds of times larger than their sum over a long row.
 //
-// What bounds it is issue slots: at 5 bits an element the memory brings 37
-// elements a clock and SM, so 3.4 lane-instructions an element are all there
-// are.  The matrix instructions are mma.sync (m16n8k16): a key tile meets 4
-// heads' two parts in 8 columns, so tcgen05's 128-row tiles with operands in
-// shared memory would spend more on writing widened codes than they save.
+// What bounds it: at 5 bits an element the memory brings 37 elements a clock
+// and SM, so 3.4 lane-instructions an element are all there are; a tile of 64
+// positions x 64 (keys and values) takes about 740, 2.9 an element, and the
+// schedulers issue in 63 of 100 clocks (with the fixed parts; the loop in 73).
+// 16 streams of 32768 positions (32 / 8 heads of 64, 336 MB) take 74.5 us, 4.5
+// TB/s, and 80 in a long run at the power cap's clocks; with the arithmetic
+// left out 61 us where the whole took 78, and the bytes alone are 51.  One
+// stream of 131072 positions takes 27.6 us for 12.8 of bytes: the list's scan
+// and the first tiles 3.5 us, the joins 6.  The matrix instructions are
+// mma.sync (m16n8k16): a key tile meets 4 heads' two parts in 8 columns, so
+// tcgen05's 128-row tiles with operands in shared memory would spend more on
+// writing widened codes than they save; the tensor pipe is busy a fifth of the
+// time.
+//
+// Tiles come by bulk copies into a ring of each warp's own, so no warp waits for
+// another before its head group ends.  (By 16-byte cp.async those 61 us are 76.)  All tiles of all streams are one list that the CTAs, and in
+// them the warps, take equal runs of; a head group that several warps share is
+// joined in shared memory, one that several CTAs share by a second kernel.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <math.h>
@@ -45,7 +58,7 @@ struct Cfg {
   static constexpr int W = NC == 1 ? 16 : 8;        // warps (128 and 255 registers a thread)
   static constexpr int NST = NC == 1 ? 2 : 4;       // stages of a warp's ring
   static constexpr int SLOT = HB * (D + 2);         // floats of a partial result (a multiple of 4)
-  static constexpr bool MAP = D >= 128;              // tiles by tensor map (swizzled)
+  static constexpr bool MAP = D == 128;             // tiles by tensor map (swizzled)
   static constexpr int SMEM = W * (NST * STAGE + SLOT * 4) + 1024;
 };
 
@@ -139,41 +152,26 @@ __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
-// Byte offset in a tile of 16-byte chunk `c` of row `r`.  Rows of 64 and 32
-// bytes lie in 128-byte lines as the tensor map's swizzle writes them (chunk
-// ^ line % 8 of the line's 8 chunks), so that the words of one chunk of 8
-// rows lie in 32 banks.
+// Byte offset in a tile of 16-byte chunk `c` of row `r`.  Rows of 64 bytes lie
+// in 128-byte lines as the tensor map's swizzle writes them (chunk ^ line % 8
+// of the line's 8 chunks), so that the words of one chunk of 8 rows lie in 32
+// banks.  Shorter rows lie as in memory: 8 rows of 32 bytes meet each bank
+// twice at most, which costs less than the swizzle's addresses (82.3 and 88.3 us for 16 x 32768).
 template <int D>
 __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
-  if constexpr (D >= 128) {
-    constexpr int R = 256 / D;  // rows a line
+  if constexpr (D == 128) {
+    constexpr int R = 2;  // rows a line
     return (r / R) * 128 + ((((r % R) * (D / 32) + c) ^ (r / R % 8)) << 4);
   }
   return r * (D / 2) + c * 16;
 }
-// Two f32 operations in one instruction.
+// a b + c of two f32 pairs in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
   asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
       "mov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
 __device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
@@ -910,10 +908,9 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
   return fn;
 }
 
-// A map over the codes as 128-byte lines (2 or 4 rows) of each head [M * nkv,
-// cap * d / 256, 128] with a box of `rows` rows: TMA moves a line a step, and
-// 64 steps for rows of 32 bytes took 4 us to fill the rings.  A box reaching
-// behind a head's last line reads zeros there.
+// A map over the codes (head dim 128) as 128-byte lines of two rows of each
+// head [M * nkv, cap / 2, 128] with a box of `rows` rows: TMA moves a line a
+// step.  A box reaching behind a head's last line reads zeros there.
 bool code_map(CUtensorMap* map, const uint8_t* base, const Kv4& kv, int rows) {
   auto fn = encode_tiled();
   if (!fn) return false;
