@@ -79,3 +79,11 @@ def test_errors_exit_1(tmp_path, capsys):
     assert cli.main(["-m", str(tmp_path / "nope.safetensors"), "--template", "t",
                      "--repack", str(tmp_path / "o.tmb"), "x"]) == 1
     assert "config.json not found" in capsys.readouterr().err
+
+
+def test_kv_bits_flag():
+    base = ["-m", "x", "--template", "t"]
+    assert cli.parse_args([*base, "p"]).kv_bits == 32
+    assert cli.parse_args([*base, "--kv-bits", "4", "p"]).kv_bits == 4
+    with pytest.raises(SystemExit):
+        cli.parse_args([*base, "--kv-bits", "8", "p"])

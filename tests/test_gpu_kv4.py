@@ -402,6 +402,98 @@ def test_attention_value_ranges(ctx, d):
         check_attention(ctx, c, q, lens)
 
 
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("n,at", [(150, 3), (150, 149), (5000, 4321)])
+@pytest.mark.parametrize("low", [False, True])
+def test_attention_far_scores(ctx, d, n, at, low):
+    # scores of up to +-1e37, one position ahead of all others by more than any
+    # rounding: its value comes back.  Tolerance: p s in two f16 parts (2^-22)
+    # against codes of up to 8 steps, p (m + 8 s) and the division with a few
+    # roundings of 2^-24, of numbers up to 3 max |v|: 2^-19 max |v|
+    rng = np.random.default_rng(d + n + at)
+    cap = (n + 3) // 4 * 4
+    for scale in (1e3, 1e7, 1e15, 1e30, 1e36):
+        q = (rng.normal(0, 1, (1, 8, d)) * scale).astype(np.float32)
+        q[0, 1] = rng.normal(0, 1, d)  # heads of one kv head far apart
+        c = filled(rng, 1, 4, d, cap, [n])
+        x = rng.normal(0, 1, (1, 4, cap, d))
+        along = np.sign(q[0, ::2])  # the first of a kv head's two heads
+        if low:
+            x = 0.1 * x - 8 * along[None, :, None]
+            x[0, :, at] = -2 * along
+        else:
+            x[0, :, at] = 8 * along
+        qc, qp = R.quantise(x.astype(np.float32))
+        qp[0, :, n:] = NAN_WORD
+        c.kc[:qc.size // 2] = dev(R.pack(qc).reshape(-1))
+        c.kp[:qp.size] = dev(qp.reshape(-1).view(np.int32))
+        out = attend(ctx, c, q, [n])
+        refs, tols = expect(c, q, [n])
+        (kc, kp), (vc, vp) = c.host()
+        v = R.values(vc[0, :, at], vp[0, :, at])
+        vmax = np.abs(R.values(vc[0, :, :n], vp[0, :, :n])).max()
+        assert np.abs(refs[0][::2] - v).max() <= 1e-9  # the premise
+        assert np.abs(out[0, ::2] - v).max() <= 2.0 ** -19 * vmax
+        k0 = R.values(kc[0, :1, :n], kp[0, :1, :n]).transpose(1, 0, 2)
+        o, A = R.attention(q[0, 1:2], k0, R.values(vc[0, :1, :n], vp[0, :1, :n]).transpose(1, 0, 2))
+        assert np.abs(out[0, 1] - o[0]).max() <= (80 * A + 128) * 2.0 ** -24 * vmax
+        assert np.isfinite(out).all()
+
+
+@pytest.mark.parametrize("d", [32, 128])
+def test_attention_queries_near_the_end_of_f32(ctx, d):
+    # |q| of 1e36 against keys of 1e-36: ordinary scores
+    rng = np.random.default_rng(d)
+    c = filled(rng, 1, 2, d, 300, [300], loud=2e-36)
+    q = (rng.normal(0, 1, (1, 8, d)) * 1e36).astype(np.float32)
+    q[0, 3] *= np.float32(1e-36)
+    check_attention(ctx, c, q, [300])
+
+
+@pytest.mark.parametrize("M", [31, 32, 33, 512, 513, 1024])
+@pytest.mark.parametrize("group", [4, 8])
+def test_attention_numbers_of_streams(ctx, M, group):
+    rng = np.random.default_rng(M)
+    lens = [int(v) for v in rng.integers(0, 200, M)]
+    lens[-1], lens[0] = 200, 0
+    c = filled(rng, M, 1, 32, 200, lens)
+    q = rng.normal(0, 1.0, (M, group, 32)).astype(np.float32)
+    out = check_attention(ctx, c, q, lens)
+    assert np.all(out[0] == 0.0)
+
+
+@pytest.mark.parametrize("d,tiles", [(64, 64), (128, 32)])
+@pytest.mark.parametrize("n_kv,group", [(1, 16), (5, 8), (80, 2), (148, 1), (149, 1)])
+def test_attention_around_the_split(ctx, d, tiles, n_kv, group):
+    # bounds of 32 and 64 tiles a head group, with and without a join
+    rng = np.random.default_rng(n_kv + d)
+    for n in (32 * tiles, 32 * tiles + 4, 64 * tiles, 64 * tiles + 4):
+        if n_kv > 80 and n > 32 * tiles + 4:
+            continue
+        c = filled(rng, 1, n_kv, d, n, [n])
+        q = rng.normal(0, 1.0, (1, n_kv * group, d)).astype(np.float32)
+        check_attention(ctx, c, q, [n])
+
+
+def test_attention_beyond_32_bit_offsets(ctx):
+    # the last streams of a cache whose codes lie beyond 2^32 bytes
+    M, n_kv, d, cap = 9, 8, 128, 1 << 20
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB free")
+    small = filled(np.random.default_rng(1), 1, n_kv, d, 2000, [2000])
+    c = Cache(M, n_kv, d, cap)
+    for big, part, w in ((c.kc, small.kc, d // 2), (c.vc, small.vc, d // 2),
+                         (c.kp, small.kp, d // 32), (c.vp, small.vp, d // 32)):
+        n = n_kv * cap * w
+        to = big[(M - 1) * n:M * n].view(n_kv, cap, w)
+        to[:, :2000] = part[:n_kv * 2000 * w].view(n_kv, 2000, w)
+    q = np.random.default_rng(2).normal(0, 1, (M, 16, d)).astype(np.float32)
+    out = attend(ctx, c, q, [0] * (M - 1) + [2000])
+    refs, tols = expect(small, q[M - 1:], [2000])
+    assert np.abs(out[M - 1] - refs[0]).max() <= tols[0]
+    assert np.all(out[:M - 1] == 0.0)
+
+
 def test_attention_nan_rows_stay_in_their_head(ctx):
     rng = np.random.default_rng(5)
     d, lens = 64, [100, 100]

@@ -250,6 +250,23 @@ def test_score(bits, T):
     m.close()
 
 
+def test_score_beyond_a_chunk():
+    # 4096 positions go through the layers at a time, 256 rows of logits; cut
+    # elsewhere, the scores agree
+    cfg = small(64, 4, 2, vocab=307)
+    m = Model.from_tensors(cfg_obj(cfg), dict(synth.make_weights(cfg, 4)))
+    toks = np.random.default_rng(8).integers(0, 307, 4500)
+    a = m.score(toks, m.new_cache(4500), top=3)
+    c = m.new_cache(4500)
+    b1, b2 = m.score(toks[:4001], c, top=3), m.score(toks[4001:], c, top=3)
+    assert c.len() == 4500
+    assert np.abs(a.logprobs[:4000] - b1.logprobs).max() < 1e-3
+    assert np.abs(a.logprobs[4001:] - b2.logprobs).max() < 1e-3
+    assert np.abs(a.entropies - np.concatenate([b1.entropies, b2.entropies])).max() < 1e-3
+    assert np.abs(a.top_logprobs - np.concatenate([b1.top_logprobs, b2.top_logprobs])).max() < 1e-3
+    m.close()
+
+
 def test_perplexity_of_a_4_bit_cache_is_near():
     # the use that the operators have together: a text scored with its cache in
     # 32 bits and in 4

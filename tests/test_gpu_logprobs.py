@@ -242,3 +242,63 @@ def test_refusals(ctx):
     assert f(ctx, P(x), 100, 0, 100, P(ids), 0, P(o), None, None, None) == 0  # no rows
     check(lib().tmg_sync(ctx), ctx)
     assert bool((o == 3.0).all())
+
+
+@pytest.mark.parametrize("rows,V,n_top", [(1, 40000, 8), (500, 3001, 20)])
+def test_captured_and_replayed_on_two_contexts(ctx, rows, V, n_top):
+    # two contexts' graphs in flight at once, each over its own buffers, replayed
+    # for new logits: the results of calls one by one
+    other = ctypes.c_void_p()
+    check(lib().tmg_create(0, None, ctypes.byref(other)))
+    rng = np.random.default_rng(rows)
+    sets = []
+    for c in (ctx, other):
+        b = dict(c=c, x=torch.zeros((rows, V), device="cuda"),
+                 t=torch.zeros(rows, dtype=torch.int32, device="cuda"),
+                 lp=torch.zeros(rows, device="cuda"), h=torch.zeros(rows, device="cuda"),
+                 ids=torch.zeros((rows, n_top), dtype=torch.int32, device="cuda"),
+                 tlp=torch.zeros((rows, n_top), device="cuda"),
+                 s=torch.cuda.ExternalStream(lib().tmg_stream(c)), g=torch.cuda.CUDAGraph())
+        torch.cuda.synchronize()
+        with torch.cuda.graph(b["g"], stream=b["s"]):
+            for _ in range(2):  # the second call finds the first one's results in place
+                check(lib().tmg_op_logprobs(c, P(b["x"]), V, rows, V, P(b["t"]), n_top, P(b["lp"]),
+                                            P(b["h"]), P(b["ids"]), P(b["tlp"])), c)
+        sets.append(b)
+    for _ in range(3):
+        host = []
+        for b in sets:
+            x = rng.normal(0, 3, (rows, V)).astype(np.float32)
+            t = rng.integers(0, V, rows)
+            b["x"].copy_(torch.from_numpy(x))
+            b["t"].copy_(torch.from_numpy(t.astype(np.int32)))
+            host.append((x, t))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for b in sets:
+                with torch.cuda.stream(b["s"]):
+                    b["g"].replay()
+        for b in sets:
+            check(lib().tmg_sync(b["c"]), b["c"])
+        for b, (x, t) in zip(sets, host):
+            one = score(ctx, x, t, n_top)
+            for name, want in zip(("lp", "h", "ids", "tlp"), one):
+                assert np.array_equal(b[name].cpu().numpy(), want)
+    for b in sets:
+        del b["g"]
+    lib().tmg_destroy(other)
+
+
+def test_offsets_beyond_32_bits(ctx):
+    # rows further apart than 2^32 bytes in all: the last ones, and a long row
+    rows, V, ld = 40, 1003, 1 << 25
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GB free")
+    assert (rows - 1) * ld * 4 > 1 << 32
+    rng = np.random.default_rng(9)
+    x = rng.normal(0, 2, (rows, V)).astype(np.float32)
+    check_rows(ctx, x, rng.integers(0, V, rows), 5, ld=ld)
+    n = 1 << 24  # one row of 16M
+    x = rng.normal(0, 2, (1, n)).astype(np.float32)
+    x[0, n - 1] = 20.0
+    check_rows(ctx, x, [n - 1], 3)

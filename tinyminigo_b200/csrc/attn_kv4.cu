@@ -184,6 +184,11 @@ struct Plan {
   bool split;     // CTAs take equal runs of tiles (else one head group each)
   float* part;    // [grid, 2] partial results
 };
+// Tiles of TK that hold n positions (n up to 2^31 - 1).
+template <int TK>
+__device__ __forceinline__ int tiles_of(int n) {
+  return int((uint32_t(n) + (TK - 1)) / TK);
+}
 __device__ __forceinline__ int clamped_len(const AttnKv4Args& a, int m) {
   return min(max(a.lens[m], 0), int(a.max_len));
 }
@@ -218,6 +223,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
   __shared__ __align__(8) uint64_t full[kWarps][C::NST];
   __shared__ int pre[kKv4MaxStreams + 1];  // tiles before each stream
   __shared__ int scan_s[kWarps];
+  __shared__ float far_s[kWarps][2][HB];
   __shared__ int slot_seg[2 * kWarps];  // head group of each warp's partials, -1: none
   const AttnKv4Args& a = pl.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -237,7 +243,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
   auto checked_tiles = [&](int m) {
     const int len = a.lens[m];
     if ((len < 0 || len > a.max_len) && a.err) atomicCAS(a.err, 0, kErrLength);
-    return (clamped_len(a, m) + TK - 1) / TK;
+    return tiles_of<TK>(clamped_len(a, m));
   };
   // this CTA's tiles [c0, c1)
   int c0, c1;
@@ -388,6 +394,22 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
             v[k][j][i] = *reinterpret_cast<const float4*>(q + h * D + j * G + t * E + 4 * i);
         }
   };
+  // Scores beyond 2^20 (in powers of two), where one rounding of a reference
+  // point would be a factor, or queries whose cq would leave f32: from there on
+  // to the head group's end x holds e - M, e the rounded exponent and M the
+  // largest so far, cq is 1 (which a product with log2 e never is) and ref
+  // counts from M.  cq (without its 2^24) and M of head h: far_s[warp][..][h].
+  auto go_far = [&]() {
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      far_s[warp][0][4 * k + t] = cq[k];
+      far_s[warp][1][4 * k + t] = ref[k];
+      if (ref[k] > -INFINITY) ref[k] = 0.f;
+      cq[k] = 1.f;
+    }
+    __syncwarp();
+  };
   auto start = [&](const float4 (&q)[NC][NG][E / 4]) {
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
@@ -429,7 +451,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
         if constexpr (E == 4) qb[k][j][2] = qb[k][j][3] = 0u;
       }
       const float un = __uint_as_float(uint32_t(254 - e) << 23);
-      cq[k] = __shfl_sync(0xffffffffu, un, src) * (a.scale * kLog2e) * 0x1p24f;
+      cq[k] = __shfl_sync(0xffffffffu, un, src) * (a.scale * kLog2e);
       ref[k] = -INFINITY;
       l[k] = 0.f;
 #pragma unroll
@@ -439,9 +461,32 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
         for (int i = 0; i < OD; ++i) o[k][j][i] = 0.f;
       }
     }
+    bool over = false;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) over |= cq[k] >= 0x1p100f;
+    if (__any_sync(0xffffffffu, over)) {
+      go_far();
+    } else {
+#pragma unroll
+      for (int k = 0; k < NC; ++k) cq[k] *= 0x1p24f;
+    }
   };
   // the sums over the lanes that share a head (each had its own positions)
   auto finish = [&]() {
+    if (cq[0] == 1.f) {  // sums relative to M, so that M alone is the reference point
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        const float f = ex2_approx(0.5f * ref[k]);
+        l[k] = l[k] * f * f;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          cm[k][j] = cm[k][j] * f * f;
+#pragma unroll
+          for (int i = 0; i < OD; ++i) o[k][j][i] = o[k][j][i] * f * f;
+        }
+        ref[k] = far_s[warp][1][4 * k + t];
+      }
+    }
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
 #pragma unroll
@@ -609,7 +654,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
       const float step = fmaxf(__uint_as_float(big << 16), 0x1p-90f);
       float p[NC][2 * KB];
       float top[NC];
-      bool grow = false;
+      bool grow = cq[0] == 1.f;
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
         top[k] = x[k][0];
@@ -620,10 +665,49 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
       if (__any_sync(0xffffffffu, grow)) {
         const float room = 12.f - float(int(__float_as_uint(step) >> 23) - 126);
 #pragma unroll
-        for (int k = 0; k < NC; ++k) {
+        for (int k = 0; k < NC; ++k)
 #pragma unroll
           for (int s = 4; s < 32; s <<= 1)
             top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], s));
+        if (cq[0] != 1.f) {
+          bool over = false;
+#pragma unroll
+          for (int k = 0; k < NC; ++k) over |= fabsf(top[k] * cq[k]) >= 0x1p20f;
+          if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+            for (int k = 0; k < NC; ++k) cq[k] *= 0x1p-24f;
+            go_far();
+          }
+        }
+        if (cq[0] == 1.f) {
+#pragma unroll
+          for (int k = 0; k < NC; ++k) {
+            const float c = far_s[warp][0][4 * k + t], was = far_s[warp][1][4 * k + t];
+            // (the order in which no product leaves f32 that e does not)
+            const float c0 = c < 1.f ? c : 0x1p24f, c1 = c < 1.f ? 0x1p24f : c;
+            auto e = [&](float x) { return __fmul_rn(__fmul_rn(x, c0), c1); };  // (no fma: M is one)
+            top[k] = e(top[k]);
+            const float M = fmaxf(was, top[k]);
+            if (M > -INFINITY) {
+              const float f = ex2_approx(was - M);
+              l[k] *= f;
+#pragma unroll
+              for (int j = 0; j < NG; ++j) {
+                cm[k][j] *= f;
+#pragma unroll
+                for (int i = 0; i < OD; ++i) o[k][j][i] *= f;
+              }
+#pragma unroll
+              for (int i = 0; i < 2 * KB; ++i) x[k][i] = e(x[k][i]) - M;
+              top[k] -= M;
+            }
+            __syncwarp();
+            far_s[warp][1][4 * k + t] = M;
+            __syncwarp();
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
           const float r = fmaxf(ref[k], fmaf(top[k], cq[k], -room)), al = ex2_approx(ref[k] - r);
           ref[k] = r;
           l[k] *= al;
@@ -805,7 +889,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_kv4_join_kernel(const Plan 
   const int warp = tid >> 5, lane = tid & 31;
   pdl_trigger();
   // everything but the partial results may be read before the main kernel ends
-  auto tiles = [&](int i) { return (clamped_len(a, i) + C::TK - 1) / C::TK; };
+  auto tiles = [&](int i) { return tiles_of<C::TK>(clamped_len(a, i)); };
   int before = 0, total = 0;
 #pragma unroll 1
   for (int i = tid; i < a.kv.M; i += kJoinThreads) {
