@@ -629,29 +629,20 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
             for (int j = 0; j < NG; ++j) pv[i][j] = 0u;
           }
       }
-      // the tile's largest step, as the lower halves of the words (a NaN step
-      // does not count)
-      uint32_t big = 0;
+      // the largest step of the lane's positions, as the words' lower halves; 2^-90
+      // at least (a NaN step is above all and fails the test below)
+      uint32_t big = 0x12801280u;
 #pragma unroll
       for (int i = 0; i < 2 * KB; ++i)
 #pragma unroll
         for (int j = 0; j < NG; j += 2)
           big = __vimax3_u16x2(big, pv[i][j], pv[i][j + 1 < NG ? j + 1 : j]);
-      big = __reduce_max_sync(0xffffffffu, big & 0xffffu);
-      if (big >= 0x7f80u) {
-        float f = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2 * KB; ++i)
-#pragma unroll
-          for (int j = 0; j < NG; ++j) f = fmaxf(f, kv4_step(pv[i][j]));
-        big = __reduce_max_sync(0xffffffffu, __float_as_uint(f)) >> 16;
-      }
 
       // p = 2^(x cq - ref), where ref is a bound of the row's exponents so far
       // plus one of its steps' less 12: p times a step stays in f16's range,
       // with 2^4 to spare before ref has to grow.  Steps below 2^-90 count as
       // that, so that sums of p stay in f32's range.
-      const float step = fmaxf(__uint_as_float(big << 16), 0x1p-90f);
+      const float step = __uint_as_float(big << 16);
       float p[NC][2 * KB];
       float top[NC];
       bool grow = cq[0] == 1.f;
@@ -663,7 +654,13 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
         grow |= !(ex2_approx(fmaf(top[k], cq[k], -ref[k])) * step <= 65000.f);
       }
       if (__any_sync(0xffffffffu, grow)) {
-        const float room = 12.f - float(int(__float_as_uint(step) >> 23) - 126);
+        float widest = 0x1p-90f;  // of all lanes; a NaN step does not count
+#pragma unroll
+        for (int i = 0; i < 2 * KB; ++i)
+#pragma unroll
+          for (int j = 0; j < NG; ++j) widest = fmaxf(widest, kv4_step(pv[i][j]));
+        const float room =
+            12.f - float(int(__reduce_max_sync(0xffffffffu, __float_as_uint(widest)) >> 23) - 126);
 #pragma unroll
         for (int k = 0; k < NC; ++k)
 #pragma unroll
@@ -879,11 +876,12 @@ template <int D, int NC>
 __global__ void __launch_bounds__(kJoinThreads) attn_kv4_join_kernel(const Plan pl, int grid) {
   using C = Cfg<D, NC>;
   constexpr int HB = C::HB, ITEMS = HB * D / 4;
-  constexpr int SL = ITEMS < kJoinThreads ? kJoinThreads / ITEMS : 1;
+  constexpr int SL = kJoinThreads / ITEMS;  // 2 or more
+  constexpr int PF = 4;                      // loads of the partials that do not wait for the weights
   extern __shared__ float fac[];  // [partial][HB] weights
   __shared__ int sums[2][kJoinThreads / 32];
   __shared__ float lsum[HB];
-  __shared__ float4 acc_s[SL > 1 ? kJoinThreads : 1];
+  __shared__ float4 acc_s[kJoinThreads];
   const AttnKv4Args& a = pl.a;
   const int VH = pl.VH, m = blockIdx.x / VH, vh = blockIdx.x - m * VH, tid = threadIdx.x;
   const int warp = tid >> 5, lane = tid & 31;
@@ -927,55 +925,73 @@ __global__ void __launch_bounds__(kJoinThreads) attn_kv4_join_kernel(const Plan 
   auto slot = [&](int i) {
     return pl.part + (int64_t(b0 + i) * 2 + (i == 0 ? first : 0)) * C::SLOT;
   };
-#pragma unroll 1
-  for (int h = warp; h < heads; h += kW) {
+  const int it = tid % ITEMS, h = it / (D / 4);
+  const bool on = h < heads;
+  float4 v[PF];
+#pragma unroll
+  for (int u = 0; u < PF; ++u) {
+    const int i = tid / ITEMS + u * SL;
+    v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (on && i < nb) v[u] = __ldcg(reinterpret_cast<const float4*>(slot(i)) + it);
+  }
+  if (warp < heads) {  // a warp a head
     float r = -INFINITY, ls = 0.f;
 #pragma unroll 1
-    for (int i = lane; i < nb; i += 32) {
-      const float v = __ldcg(slot(i) + HB * D + h), l = __ldcg(slot(i) + HB * D + HB + h);
-      fac[i * HB + h] = v;
-      // (the sum so far moves with the reference point)
-      const float n = fmaxf(r, v);
-      ls = fmaf(ls, ex2_approx(r - n), l * ex2_approx(v - n));
-      r = n;
+    for (int base = lane; base < nb; base += 32 * PF) {
+      float x[PF], l[PF];
+#pragma unroll
+      for (int u = 0; u < PF; ++u) {
+        const int i = base + 32 * u;
+        x[u] = -INFINITY, l[u] = 0.f;
+        if (i < nb) {
+          x[u] = __ldcg(slot(i) + HB * D + warp);
+          l[u] = __ldcg(slot(i) + HB * D + HB + warp);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < PF; ++u) {
+        const int i = base + 32 * u;
+        if (i >= nb) break;
+        fac[i * HB + warp] = x[u];
+        // (the sum so far moves with the reference point)
+        const float n = fmaxf(r, x[u]);
+        ls = fmaf(ls, ex2_approx(r - n), l[u] * ex2_approx(x[u] - n));
+        r = n;
+      }
     }
     const float top = warp_max(r);
     ls = warp_sum(lane < nb ? ls * ex2_approx(r - top) : 0.f);
 #pragma unroll 1
-    for (int i = lane; i < nb; i += 32) fac[i * HB + h] = ex2_approx(fac[i * HB + h] - top);
-    if (lane == 0) lsum[h] = ls;
+    for (int i = lane; i < nb; i += 32) fac[i * HB + warp] = ex2_approx(fac[i * HB + warp] - top);
+    if (lane == 0) lsum[warp] = ls;
   }
   __syncthreads();
-  for (int it = tid % ITEMS; it < heads * (D / 4); it += kJoinThreads) {
-    const int h = it / (D / 4);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = SL > 1 ? tid / ITEMS : 0; i < nb; i += SL) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(i)) + it);
-      const float f = fac[i * HB + h];
-      acc.x = fmaf(v.x, f, acc.x);
-      acc.y = fmaf(v.y, f, acc.y);
-      acc.z = fmaf(v.z, f, acc.z);
-      acc.w = fmaf(v.w, f, acc.w);
-    }
-    if constexpr (SL > 1) acc_s[tid] = acc;
-    else {
-      const float f = 1.0f / lsum[h];
-      reinterpret_cast<float4*>(out)[it] = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
-    }
-  }
-  if constexpr (SL > 1) {
-    __syncthreads();
-    if (tid < heads * (D / 4)) {
-      float4 acc = acc_s[tid];
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](const float4& v, int i) {
+    const float f = fac[i * HB + h];
+    acc.x = fmaf(v.x, f, acc.x);
+    acc.y = fmaf(v.y, f, acc.y);
+    acc.z = fmaf(v.z, f, acc.z);
+    acc.w = fmaf(v.w, f, acc.w);
+  };
+  if (on) {
 #pragma unroll
-      for (int s = 1; s < SL; ++s) {
-        const float4 v = acc_s[s * ITEMS + tid];
-        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-      }
-      const float f = 1.0f / lsum[tid / (D / 4)];
-      reinterpret_cast<float4*>(out)[tid] = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+    for (int u = 0; u < PF; ++u)
+      if (tid / ITEMS + u * SL < nb) add(v[u], tid / ITEMS + u * SL);
+#pragma unroll 8
+    for (int i = tid / ITEMS + PF * SL; i < nb; i += SL)
+      add(__ldcg(reinterpret_cast<const float4*>(slot(i)) + it), i);
+  }
+  acc_s[tid] = acc;
+  __syncthreads();
+  if (tid < ITEMS && on) {
+#pragma unroll
+    for (int s = 1; s < SL; ++s) {
+      const float4 o = acc_s[s * ITEMS + tid];
+      acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
     }
+    const float f = 1.0f / lsum[h];
+    reinterpret_cast<float4*>(out)[it] = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
   }
 }
 
