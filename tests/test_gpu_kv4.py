@@ -462,6 +462,13 @@ def test_attention_numbers_of_streams(ctx, M, group):
     assert np.all(out[0] == 0.0)
 
 
+@pytest.mark.parametrize("M", [3, 40, 1024])
+def test_attention_of_empty_streams(ctx, M):
+    c = Cache(M, 2, 64, 4096)  # nothing written: NaN parameters
+    q = np.random.default_rng(M).normal(0, 1, (M, 4, 64)).astype(np.float32)
+    assert np.all(attend(ctx, c, q, [0] * M) == 0.0)
+
+
 @pytest.mark.parametrize("d,tiles", [(64, 64), (128, 32)])
 @pytest.mark.parametrize("n_kv,group", [(1, 16), (5, 8), (80, 2), (148, 1), (149, 1)])
 def test_attention_around_the_split(ctx, d, tiles, n_kv, group):

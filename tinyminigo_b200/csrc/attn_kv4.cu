@@ -867,42 +867,75 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
   }
 }
 
-// The head groups that several CTAs shared, joined from the workspace (one
-// CTA each), and zeros for empty streams.  A thread takes 4 columns of one
-// head of every SL-th partial result, so that their loads are in flight
-// together.
+// The head groups that several CTAs shared, joined from the workspace, and
+// zeros for empty streams.  A CTA a head group; or, for MANY of them, CTA b
+// takes the one that begins in the main kernel's CTA b and goes on behind it.
+// A thread takes 4 columns of one head of every SL-th partial result, so that
+// their loads are in flight together.
 constexpr int kJoinThreads = 512;
-template <int D, int NC>
+template <int D, int NC, bool MANY>
 __global__ void __launch_bounds__(kJoinThreads) attn_kv4_join_kernel(const Plan pl, int grid) {
   using C = Cfg<D, NC>;
   constexpr int HB = C::HB, ITEMS = HB * D / 4;
   constexpr int SL = kJoinThreads / ITEMS;  // 2 or more
   constexpr int PF = 4;                      // loads of the partials that do not wait for the weights
   extern __shared__ float fac[];  // [partial][HB] weights
-  __shared__ int sums[2][kJoinThreads / 32];
+  __shared__ int sums[2][kJoinThreads / 32], at_s[3];
   __shared__ float lsum[HB];
   __shared__ float4 acc_s[kJoinThreads];
   const AttnKv4Args& a = pl.a;
-  const int VH = pl.VH, m = blockIdx.x / VH, vh = blockIdx.x - m * VH, tid = threadIdx.x;
-  const int warp = tid >> 5, lane = tid & 31;
-  pdl_trigger();
-  // everything but the partial results may be read before the main kernel ends
-  auto tiles = [&](int i) { return tiles_of<C::TK>(clamped_len(a, i)); };
-  int before = 0, total = 0;
-#pragma unroll 1
-  for (int i = tid; i < a.kv.M; i += kJoinThreads) {
-    const int n = tiles(i);
-    total += n;
-    if (i < m) before += n;
-  }
-  const int nt = tiles(m);
-  before = __reduce_add_sync(0xffffffffu, before);
-  total = __reduce_add_sync(0xffffffffu, total);
-  if (lane == 0) sums[0][warp] = before, sums[1][warp] = total;
-  __syncthreads();
+  const int VH = pl.VH, M = a.kv.M, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int kW = kJoinThreads / 32;
-  before = __reduce_add_sync(0xffffffffu, lane < kW ? sums[0][lane % kW] : 0);
-  total = __reduce_add_sync(0xffffffffu, lane < kW ? sums[1][lane % kW] : 0) * VH;
+  pdl_trigger();
+  // everything but the partial results may be read before the main kernel ends:
+  // the stream m, its tiles and those before it, and all
+  auto tiles = [&](int i) { return tiles_of<C::TK>(clamped_len(a, i)); };
+  int m, nt, before = 0, total = 0, T = 0;
+  if constexpr (MANY) {
+    // two streams a thread, scanned over the CTA; the one that holds the first
+    // tile behind main CTA b's
+    static_assert(kKv4MaxStreams <= 2 * kJoinThreads);
+    const int n0 = 2 * tid < M ? tiles(2 * tid) : 0, n1 = 2 * tid + 1 < M ? tiles(2 * tid + 1) : 0;
+    int at = n0 + n1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += v;
+    }
+    if (lane == 31) sums[0][warp] = at;
+    __syncthreads();
+    const int of_warp = lane < kW ? sums[0][lane % kW] : 0;
+    total = __reduce_add_sync(0xffffffffu, of_warp) * VH;
+    at += __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0) - n0 - n1;
+    pdl_wait();
+    for (int i = blockIdx.x; i < M; i += gridDim.x)
+      if (tiles(i) == 0)
+        for (int j = tid; j < a.nq * D; j += kJoinThreads) a.out[int64_t(i) * a.out_ld + j] = 0.f;
+    if (int(blockIdx.x) + 1 >= min(grid, total)) return;
+    T = Deal(total, min(grid, total)).first(blockIdx.x + 1);
+    if (T >= at * VH && T < (at + n0 + n1) * VH) {
+      const bool second = T >= (at + n0) * VH;
+      at_s[0] = 2 * tid + second, at_s[1] = second ? at + n0 : at, at_s[2] = second ? n1 : n0;
+    }
+    __syncthreads();
+    m = at_s[0], before = at_s[1], nt = at_s[2];
+  } else {
+    m = blockIdx.x / VH;
+#pragma unroll 1
+    for (int i = tid; i < M; i += kJoinThreads) {
+      const int n = tiles(i);
+      total += n;
+      if (i < m) before += n;
+    }
+    nt = tiles(m);
+    before = __reduce_add_sync(0xffffffffu, before);
+    total = __reduce_add_sync(0xffffffffu, total);
+    if (lane == 0) sums[0][warp] = before, sums[1][warp] = total;
+    __syncthreads();
+    before = __reduce_add_sync(0xffffffffu, lane < kW ? sums[0][lane % kW] : 0);
+    total = __reduce_add_sync(0xffffffffu, lane < kW ? sums[1][lane % kW] : 0) * VH;
+  }
+  const int vh = MANY ? (T - before * VH) / nt : int(blockIdx.x) - m * VH;
   const int per = a.nq / a.kv.nkv, g0 = (vh & ((1 << pl.gsh) - 1)) * pl.gh;
   const int heads = min(pl.gh, per - g0);
   float* out = a.out + int64_t(m) * a.out_ld + int64_t((vh >> pl.gsh) * per + g0) * D;
@@ -914,14 +947,18 @@ __global__ void __launch_bounds__(kJoinThreads) attn_kv4_join_kernel(const Plan 
     nb = deal.owner(s0 + nt - 1) - b0 + 1;
     // only the first of the CTAs can have begun before this head group
     first = s0 <= deal.first(b0) ? 0 : 1;
+    // (T may be a head group's first tile, or an earlier CTA's head group)
+    if (MANY && (s0 == T || b0 != int(blockIdx.x))) return;
   }
-  pdl_wait();
-  if (nt == 0) {
+  if constexpr (!MANY) {
+    pdl_wait();
+    if (nt == 0) {
 #pragma unroll 1
-    for (int i = tid; i < heads * D; i += kJoinThreads) out[i] = 0.f;
-    return;
+      for (int i = tid; i < heads * D; i += kJoinThreads) out[i] = 0.f;
+      return;
+    }
+    if (nb == 1) return;
   }
-  if (nb == 1) return;
   auto slot = [&](int i) {
     return pl.part + (int64_t(b0 + i) * 2 + (i == 0 ? first : 0)) * C::SLOT;
   };
@@ -1066,13 +1103,20 @@ cudaError_t run(const AttnKv4Args& a, cudaStream_t s) {
   const int grid = pl.split ? a.num_sms : int(groups);
   TMG_CUDA_TRY(launch(attn_kv4_kernel<D, NC>, grid, C::W * 32, C::SMEM, s, km, vm, pl));
   if (!pl.split) return cudaSuccess;
-  return launch(attn_kv4_join_kernel<D, NC>, int(groups), kJoinThreads, grid * C::HB * 4, s, pl, grid);
+  // Streams of up to 300 positions, 8 heads of 64, all in all: 800 head groups 20.3
+  // us with a CTA each and 20.1 by main CTAs, 2048: 33.3 and 27.8, 8192: 91 and 57;
+  // 192: 11.2 and 12.2
+  if (groups > 4 * grid)
+    return launch(attn_kv4_join_kernel<D, NC, true>, grid, kJoinThreads, grid * C::HB * 4, s, pl, grid);
+  return launch(attn_kv4_join_kernel<D, NC, false>, int(groups), kJoinThreads, grid * C::HB * 4, s, pl,
+                grid);
 }
 
 template <int D, int NC>
 cudaError_t prepare() {
   TMG_CUDA_TRY(set_carveout(attn_kv4_kernel<D, NC>, Cfg<D, NC>::SMEM));
-  return set_carveout(attn_kv4_join_kernel<D, NC>);
+  TMG_CUDA_TRY((set_carveout(attn_kv4_join_kernel<D, NC, true>)));
+  return set_carveout(attn_kv4_join_kernel<D, NC, false>);
 }
 
 int column_tiles(int per) {
