@@ -470,7 +470,8 @@ def test_attention_of_empty_streams(ctx, M):
 
 
 @pytest.mark.parametrize("d,tiles", [(64, 64), (128, 32)])
-@pytest.mark.parametrize("n_kv,group", [(1, 16), (5, 8), (80, 2), (148, 1), (149, 1)])
+@pytest.mark.parametrize("n_kv,group", [(1, 16), (5, 8), (80, 2), (148, 1), (149, 1),
+                                        (197, 1), (198, 1)])
 def test_attention_around_the_split(ctx, d, tiles, n_kv, group):
     # bounds of 32 and 64 tiles a head group, with and without a join
     rng = np.random.default_rng(n_kv + d)

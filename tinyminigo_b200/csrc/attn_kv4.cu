@@ -1098,8 +1098,13 @@ cudaError_t run(const AttnKv4Args& a, cudaStream_t s) {
   // join and what prepares it cost about 4 us, so up to 32 tiles a head group
   // (2 a warp; 64 where the head groups fill the GPU by half) go without.
   // 2048 positions of 8 heads of 64: 10.2 and 10.6 us; 4096: 14.8 and 10.9; 128
-  // groups of 2048 (heads of 128): 16.4 and 20.5 us.
-  pl.split = groups > a.num_sms || a.max_len > (2 * groups > a.num_sms ? 64 : 32) * C::TK;
+  // groups of 2048 (heads of 128): 16.4 and 20.5 us.  So do a few more head
+  // groups than SMs, where one column tile makes them short: 192 of up to 300
+  // positions (heads of 64) 8.9 and 11.2 us, of up to 2000 15.5 and 17.7; 256 of
+  // up to 300 11.8 and 10.7.
+  const int64_t most = NC == 1 ? a.num_sms + a.num_sms / 3 : a.num_sms;
+  const bool half_full = 2 * groups > a.num_sms && groups <= a.num_sms;
+  pl.split = groups > most || a.max_len > (half_full ? 64 : 32) * C::TK;
   const int grid = pl.split ? a.num_sms : int(groups);
   TMG_CUDA_TRY(launch(attn_kv4_kernel<D, NC>, grid, C::W * 32, C::SMEM, s, km, vm, pl));
   if (!pl.split) return cudaSuccess;
