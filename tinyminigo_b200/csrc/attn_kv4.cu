@@ -15,13 +15,13 @@
 //
 // What bounds it: at 5 bits an element the memory brings 37 elements a clock
 // and SM, so 3.4 lane-instructions an element are all there are; a tile of 64
-// positions x 64 (keys and values) takes about 740, 2.9 an element, and the
+// positions x 64 (keys and values) takes about 730, 2.9 an element, and the
 // schedulers issue in 63 of 100 clocks (with the fixed parts; the loop in 73).
-// 16 streams of 32768 positions (32 / 8 heads of 64, 336 MB) take 74.5 us, 4.5
-// TB/s, and 80 in a long run at the power cap's clocks; with the arithmetic
+// 16 streams of 32768 positions (32 / 8 heads of 64, 336 MB) take 72 us, 4.7
+// TB/s, and 79 in a long run at the power cap's clocks; with the arithmetic
 // left out 61 us where the whole took 78, and the bytes alone are 51.  One
-// stream of 131072 positions takes 27.6 us for 12.8 of bytes: the list's scan
-// and the first tiles 3.5 us, the joins 6.  The matrix instructions are
+// stream of 131072 positions takes 26 us for 12.8 of bytes: the list's scan
+// and the first tiles 3.5 us, the joins 5.  The matrix instructions are
 // mma.sync (m16n8k16): a key tile meets 4 heads' two parts in 8 columns, so
 // tcgen05's 128-row tiles with operands in shared memory would spend more on
 // writing widened codes than they save; the tensor pipe is busy a fifth of the

@@ -14,11 +14,11 @@
 // the few threads whose second value reaches it, which alone are read again.
 //
 // It is bound by the one read of the logits: 2047 rows of 128256 (1.05 GB) take
-// 168 us, 6.25 TB/s, 95% of a plain copy's rate, with 8 alternatives and 182
-// with 64; in a long run at the power cap's clocks 187.  By 16-byte loads, four
+// 167 us, 6.3 TB/s, 96% of a plain copy's rate, with 8 alternatives and 182
+// with 64; in a long run at the power cap's clocks 184.  By 16-byte loads, four
 // of them in flight a thread; through a ring of bulk copies in shared memory it
-// took 232 us.  One row of 128256 takes 8.5 us by the host's clock (a cluster of
-// 8 CTAs; one CTA 24.9), little above a launch.
+// took 232 us.  One row of 128256 takes 6.6 us (a cluster of 8 CTAs; of 4 7.2,
+// one CTA 24.9).
 #include <cooperative_groups.h>
 #include <math.h>
 
