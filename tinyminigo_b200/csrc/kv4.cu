@@ -9,7 +9,7 @@
 // goes 16 bytes a lane, a warp's 512 in one piece; several units a warp, their
 // loads in flight together, once there are enough rows to fill the GPU so.
 //
-// Reading 65536 rows (8 heads of 128: 84 MB of cache, 537 MB of f32) takes 98.4
+// Reading 65536 rows (8 heads of 128: 84 MB of cache, 537 MB of f32) takes 98
 // us, 6.3 TB/s, 96% of a plain copy's rate.  Writing 4000 rows (32.8 MB in, 5.1
 // MB out) takes 13.5 us, where the bytes are 5.8: two waves of blocks that each
 // load, meet the group's extremes by 3 shuffles and store, at 183 instructions
