@@ -441,7 +441,8 @@ int tmg_op_kv4_read(tmg_ctx* ctx, const tmg_kv4* kv, const int32_t* pos, const i
                     int64_t T, float* k, float* v, int64_t row_ld);
 /* Decode attention over the cache, as tmg_op_attn_decode over f32 rows: for
  * each stream m one query row q + m * q_ld of n_q heads over its first
- * lens[m] positions, to out + m * out_ld (a stream of length 0 gets zeros).
+ * lens[m] positions, to out + m * out_ld (a stream of length 0 gets zeros;
+ * out may be q, with the same leading dimension).
  * At most 16 query heads per kv head.  max_len: a bound of all lengths that
  * the caller knows (the capacity if none), which sizes the split; a length
  * outside [0, max_len] is taken as the nearer end (TMG_ERR_INVALID).  ws: at

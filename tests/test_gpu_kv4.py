@@ -517,6 +517,40 @@ def test_attention_nan_rows_stay_in_their_head(ctx):
     assert nan[1, :4, 32:].all() and not nan[1, :4, :32].any() and not nan[1, 4:].any()
 
 
+@pytest.mark.parametrize("n", [92, 6000])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_attention_bad_queries_stay_in_their_head(ctx, n, value):
+    rng = np.random.default_rng(n)
+    for d, group in ((64, 4), (128, 8)):
+        c = filled(rng, 2, 2, d, n, [n, n])
+        q = rng.normal(0, 1, (2, 2 * group, d)).astype(np.float32)
+        clean = attend(ctx, c, q, [n, n])
+        q[1, 1, 7] = value
+        out = attend(ctx, c, q, [n, n])
+        refs, tols = expect(c, np.where(np.isfinite(q), q, 0), [n, n])
+        assert np.isnan(out[1, 1]).all() and np.array_equal(out[0], clean[0])
+        rest = [h for h in range(2 * group) if h != 1]
+        assert np.abs(out[1, rest] - refs[1][rest]).max() <= tols[1]
+
+
+def test_attention_over_its_own_query(ctx):
+    # out may be q: a head group's query is read before its output is written
+    rng = np.random.default_rng(3)
+    for M, n, d in ((2, 300, 64), (3, 20000, 64), (40, 700, 128)):
+        lens = [int(v) for v in rng.integers(0, n, M)]
+        lens[0] = n
+        c = filled(rng, M, 2, d, (n + 3) // 4 * 4, lens)
+        q = rng.normal(0, 1, (M, 8, d)).astype(np.float32)
+        want = attend(ctx, c, q, lens)
+        x, ln = dev(q.reshape(M, 8 * d)), dev(np.asarray(lens, np.int32))
+        ws, size = workspace(ctx, c, 8)
+        torch.cuda.synchronize()
+        check(lib().tmg_op_attn_decode_kv4(ctx, c.ref(), P(x), 8 * d, P(ln), c.cap, 8, P(x), 8 * d,
+                                           P(ws), size), ctx)
+        check(lib().tmg_sync(ctx), ctx)
+        assert np.array_equal(x.cpu().numpy().reshape(M, 8, d), want)
+
+
 def test_attention_length_out_of_range(ctx):
     rng = np.random.default_rng(6)
     c = filled(rng, 2, 2, 64, 64, [64, 64])
