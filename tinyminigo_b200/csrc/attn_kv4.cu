@@ -59,6 +59,7 @@ struct Cfg {
   static constexpr int NST = NC == 1 ? 2 : 4;       // stages of a warp's ring
   static constexpr int SLOT = HB * (D + 2);         // floats of a partial result (a multiple of 4)
   static constexpr bool MAP = D == 128;             // tiles by tensor map (swizzled)
+  static constexpr int WPL = TK * NG / 32;          // a lane's share of a tile's parameter words
   static constexpr int SMEM = W * (NST * STAGE + SLOT * 4) + 1024;
 };
 
@@ -66,6 +67,12 @@ struct Cfg {
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 1 / x by the SFU's rcp instruction (relative error about 2^-23)
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -130,6 +137,16 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
   return v;
 }
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds8(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=h"(v) : "r"(a));
+  return v;
+}
 template <int N>
 __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[N]) {
   if constexpr (N == 4)
@@ -176,13 +193,29 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 __device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
 
+// A head group's window: a power of two 2^K, as its bf16 pattern (K + 127) << 7, such
+// that the steps s and minima m of its values so far have s <= 2^K, |m| <= 2^(K +
+// kMinima), K from kLeast to kFar.  Weights are scaled so that p 2^K is at most 2^16, thus p s
+// fits f16; sums of p |m| stay below 2^(16 + 36) a position, those of p below 2^106.
+constexpr int kMinima = 36, kLeast = -90, kFar = 20;
+constexpr int kNoWindow = 0x7fff;  // no value passes it
+__device__ __forceinline__ int window_of(int K) { return (K + 127) << 7; }
+// The window that steps up to s_max and minima up to m_max (as bf16 patterns) fit:
+// `now` if it does, else one with some room for larger steps.
+__device__ __forceinline__ int fit_window(int now, int s_max, int m_max) {
+  if (s_max <= now && m_max <= now + (kMinima << 7)) return now;
+  const int least = max(max((s_max + 0x7f) & ~0x7f, ((m_max + 0x7f) & ~0x7f) - (kMinima << 7)),
+                        window_of(kLeast));
+  return least <= window_of(kFar) ? min(least + (3 << 7), window_of(kFar)) : kNoWindow;
+}
+
 // The tiles of all streams, in order of (stream, head group, tile).
 struct Plan {
   AttnKv4Args a;
   int gh, gsh;    // query heads a head group; log2 of a kv head's head groups
   int VH;         // head groups a stream
   bool split;     // CTAs take equal runs of tiles (else one head group each)
-  float* part;    // [grid, 2] partial results
+  float* part;    // [grid, 2] partial results: weighted means, reference points, sums of weights
 };
 // Tiles of TK that hold n positions (n up to 2^31 - 1).
 template <int TK>
@@ -210,6 +243,97 @@ struct Cursor {
   int m, vh, tile, nt;
 };
 
+// Wide mode: values that no window holds (steps or minima of one tile far apart,
+// or near the ends of f32).  From there on to the head group's end p is at most 1,
+// cm is 0 and o counts in units of 2^unit[head][group], a bound of p |v| so far, to
+// which each product goes as a 64-bit number; so it is as exact as 32-bit sums, and
+// neither |v| nor what p leaves of it can leave f32.  A function of its own, called
+// for such tiles only: in the loop its registers would cost every tile (8 heads of
+// 128 a kv head: 130 us and not 115).
+template <int D, int NC>
+struct Wide {
+  using C = Cfg<D, NC>;
+  static constexpr int NG = C::NG, KB = C::TK / 16, OD = D == 16 ? 2 : 4;
+  float x[NC][2 * KB], cq[NC], ref[NC], l[NC], cm[NC][NG], o[NC][NG][OD];
+  float shift[NC];  // log2 of what the sums so far are multiplied by
+};
+template <int D, int NC>
+__device__ __noinline__ void wide_tile(Wide<D, NC>& w, int (*unit)[Cfg<D, NC>::NG], uint32_t base,
+                                       int valid, bool first) {
+  using C = Cfg<D, NC>;
+  constexpr int NG = C::NG, KB = C::TK / 16, OD = D == 16 ? 2 : 4;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  __syncwarp();
+#pragma unroll 1
+  for (int k = 0; k < NC; ++k) {
+    const float al = ex2_approx(w.shift[k]);
+    w.l[k] *= al;
+#pragma unroll
+    for (int i = 0; i < 2 * KB; ++i) {
+      w.x[k][i] = ex2_approx(fmaf(w.x[k][i], w.cq[k], -w.ref[k]));  // p from here on
+      w.l[k] += w.x[k][i];
+    }
+#pragma unroll 1
+    for (int j = 0; j < NG; ++j) {
+      float o[OD];
+#pragma unroll
+      for (int i = 0; i < OD; ++i) o[i] = w.o[k][j][i];
+      int e = unit[4 * k + t][j];
+      if (first) {  // o and cm as the other tiles left them
+        float c = w.cm[k][j], big = 0.f;
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) c += __shfl_xor_sync(0xffffffffu, c, s);
+#pragma unroll
+        for (int i = 0; i < OD; ++i) big = fmaxf(big, fabsf(o[i] += c));
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
+        e = big > 0.f ? ilogbf(big) + 1 : -4000;
+#pragma unroll
+        for (int i = 0; i < OD; ++i) o[i] = scalbnf(o[i], -e);
+      }
+      // times 2^shift
+      const float whole = floorf(w.shift[k]);
+      const float part = w.shift[k] <= -4000.f ? 0.f : ex2_approx(w.shift[k] - whole);
+      e = max(e + int(fmaxf(whole, -4000.f)), -4000);
+      // the exponent above the largest p |v| of the tile
+      int up = e;
+#pragma unroll 1
+      for (int i = 0; i < 2 * KB; ++i) {
+        const uint32_t par = 8 * i + g < valid
+            ? lds32(base + 2 * C::CODE + C::PAR + ((8 * i + g) * NG + j) * 4) : 0u;
+        const double m = kv4_min(par), s = kv4_step(par);
+        const double y = double(w.x[k][i]) * fmax(fabs(m), fabs(fma(15.0, s, m)));
+        if (y > 0.0) up = max(up, (__double2hiint(y) >> 20) - 1022);
+      }
+#pragma unroll
+      for (int s = 4; s < 32; s <<= 1) up = max(up, __shfl_xor_sync(0xffffffffu, up, s));
+#pragma unroll
+      for (int i = 0; i < OD; ++i) o[i] = scalbnf(o[i] * part, e - up);
+      const double to_unit = __hiloint2double((1023 - max(up, -1000)) << 20, 0);
+#pragma unroll 1
+      for (int i = 0; i < 2 * KB; ++i)
+#pragma unroll 1
+        for (int r = 8 * i; r < min(8 * i + 8, valid); ++r) {
+          const double p =
+              double(__shfl_sync(0xffffffffu, w.x[k][i], 4 * (r & 7) + t)) * to_unit;
+          const uint32_t par = lds32(base + 2 * C::CODE + C::PAR + (r * NG + j) * 4);
+          uint32_t codes;
+          if constexpr (D == 16) codes = lds8(base + C::CODE + r * 8 + g);
+          else codes = lds16(base + C::CODE + chunk_off<D>(r, j) + 2 * g);
+#pragma unroll
+          for (int n = 0; n < OD; ++n)
+            o[n] += float(p * double(fmaf(float(codes >> (4 * n) & 15u), kv4_step(par),
+                                          kv4_min(par))));
+        }
+#pragma unroll
+      for (int i = 0; i < OD; ++i) w.o[k][j][i] = o[i];
+      __syncwarp();
+      if (g == 0) unit[4 * k + t][j] = up;
+    }
+  }
+  __syncwarp();
+}
+
 template <int D, int NC>
 __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
     attn_kv4_kernel(const __grid_constant__ CUtensorMap kmap,
@@ -224,6 +348,10 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
   __shared__ int pre[kKv4MaxStreams + 1];  // tiles before each stream
   __shared__ int scan_s[kWarps];
   __shared__ float far_s[kWarps][2][HB];
+  // a head group's window as bounds (set_window), and as it is
+  __shared__ __align__(16) uint32_t bounds_s[kWarps][2];
+  __shared__ int window_s[kWarps];
+  __shared__ int unit_s[kWarps][HB][NG];  // exponents of o (wide mode)
   __shared__ int slot_seg[2 * kWarps];  // head group of each warp's partials, -1: none
   const AttnKv4Args& a = pl.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -410,6 +538,17 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
     }
     __syncwarp();
   };
+  // The head group's window, and whether the next tile is tested against it (else it is off).
+  auto set_window = [&](int now, bool test) {
+    const int w = test ? now : kNoWindow;
+    __syncwarp();
+    if (lane == 0) {
+      bounds_s[warp][0] = w * 0x10001u + (kMinima << 23);
+      bounds_s[warp][1] = __float_as_uint(w == kNoWindow ? -INFINITY : 15.98f + 127 - (w >> 7));
+      window_s[warp] = now;
+    }
+    __syncwarp();
+  };
   auto start = [&](const float4 (&q)[NC][NG][E / 4]) {
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
@@ -461,6 +600,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
         for (int i = 0; i < OD; ++i) o[k][j][i] = 0.f;
       }
     }
+    set_window(window_of(kLeast), false);
     bool over = false;
 #pragma unroll
     for (int k = 0; k < NC; ++k) over |= cq[k] >= 0x1p100f;
@@ -471,22 +611,11 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
       for (int k = 0; k < NC; ++k) cq[k] *= 0x1p24f;
     }
   };
-  // the sums over the lanes that share a head (each had its own positions)
+  // the sums over the lanes that share a head (each had its own positions): o
+  // becomes the weighted mean of the values, which f32 holds whatever they are
   auto finish = [&]() {
-    if (cq[0] == 1.f) {  // sums relative to M, so that M alone is the reference point
-#pragma unroll
-      for (int k = 0; k < NC; ++k) {
-        const float f = ex2_approx(0.5f * ref[k]);
-        l[k] = l[k] * f * f;
-#pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          cm[k][j] = cm[k][j] * f * f;
-#pragma unroll
-          for (int i = 0; i < OD; ++i) o[k][j][i] = o[k][j][i] * f * f;
-        }
-        ref[k] = far_s[warp][1][4 * k + t];
-      }
-    }
+    __syncwarp();
+    const bool wide = window_s[warp] == kNoWindow;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
 #pragma unroll
@@ -495,10 +624,33 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
 #pragma unroll
         for (int j = 0; j < NG; ++j) cm[k][j] += __shfl_xor_sync(0xffffffffu, cm[k][j], s);
       }
+      const float f = rcp_approx(l[k]);
 #pragma unroll
       for (int j = 0; j < NG; ++j)
 #pragma unroll
-        for (int i = 0; i < OD; ++i) o[k][j][i] += cm[k][j];
+        for (int i = 0; i < OD; ++i) {
+          o[k][j][i] = (o[k][j][i] + cm[k][j]) * f;
+        }
+    }
+    if (wide) {
+#pragma unroll
+      for (int k = 0; k < NC; ++k)
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          const int e = max(unit_s[warp][4 * k + t][j], -252), h = e >> 1;
+#pragma unroll
+          for (int i = 0; i < OD; ++i)
+            o[k][j][i] = o[k][j][i] * __int_as_float((h + 127) << 23) *
+                         __int_as_float((e - h + 127) << 23);
+        }
+    }
+    if (cq[0] == 1.f) {  // sums relative to M, so that M alone is the reference point
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        const float f = ex2_approx(0.5f * ref[k]);
+        l[k] = l[k] * f * f;
+        ref[k] = far_s[warp][1][4 * k + t];
+      }
     }
   };
   auto write_out = [&](const Cursor& c) {
@@ -508,11 +660,6 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
     for (int k = 0; k < NC; ++k) {
       const int h = 4 * k + t;
       if (h >= heads) continue;
-      const float f = 1.0f / l[k];
-#pragma unroll
-      for (int j = 0; j < NG; ++j)
-#pragma unroll
-        for (int i = 0; i < OD; ++i) o[k][j][i] *= f;
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         float* p = out + h * D + j * G + g * OD;
@@ -619,6 +766,11 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
 #pragma unroll
       for (int i = 0; i < 2 * KB; ++i)
         lds_words<NG>(base + 2 * C::CODE + C::PAR + (8 * i + g) * NG * 4, pv[i]);
+      // a share of them: word i is of position (lane WPL + i) / NG, group i % NG
+      uint32_t pw[C::WPL];
+      lds_words<C::WPL>(base + 2 * C::CODE + C::PAR + lane * C::WPL * 4, pw);
+      uint32_t bounds[2];
+      lds_words<2>(smem_u32(bounds_s[warp]), bounds);
       if (valid < TK) {
 #pragma unroll
         for (int i = 0; i < 2 * KB; ++i)
@@ -628,39 +780,54 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
 #pragma unroll
             for (int j = 0; j < NG; ++j) pv[i][j] = 0u;
           }
+#pragma unroll
+        for (int i = 0; i < C::WPL; ++i)
+          if ((lane * C::WPL + i) / NG >= valid) pw[i] = bounds[0] & 0xffffu;  // m = 0, s = 2^K
       }
-      // the largest step of the lane's positions, as the words' lower halves; 2^-90
-      // at least (a NaN step is above all and fails the test below)
-      uint32_t big = 0x12801280u;
-#pragma unroll
-      for (int i = 0; i < 2 * KB; ++i)
-#pragma unroll
-        for (int j = 0; j < NG; j += 2)
-          big = __vimax3_u16x2(big, pv[i][j], pv[i][j + 1 < NG ? j + 1 : j]);
 
-      // p = 2^(x cq - ref), where ref is a bound of the row's exponents so far
-      // plus one of its steps' less 12: p times a step stays in f16's range,
-      // with 2^4 to spare before ref has to grow.  Steps below 2^-90 count as
-      // that, so that sums of p stay in f32's range.
-      const float step = __uint_as_float(big << 16);
+      // p = 2^(x cq - ref), where ref is a bound of the row's exponents so far plus K
+      // less 12: p times a step stays in f16's range, with 2^4 to spare before ref has
+      // to grow.  The tile's parameters are held against the window (fit_window) as
+      // pairs of 16 bits, signed and unsigned: the unsigned maximum has the steps' and
+      // the largest negative minimum, the signed one the largest positive minimum.  A
+      // NaN step is above all.
+      uint32_t most = __vmaxu2(pw[0], pw[1]), most_s = __vmaxs2(pw[0], pw[1]);
+      if constexpr (C::WPL == 4) {
+        most = __vimax3_u16x2(most, pw[2], pw[3]);
+        most_s = __vimax3_s16x2(most_s, pw[2], pw[3]);
+      }
+      const bool off = __vimax3_s16x2(most & 0x7fffffffu, most_s, bounds[0]) != bounds[0];
       float p[NC][2 * KB];
       float top[NC];
-      bool grow = cq[0] == 1.f;
+      bool grow = off || cq[0] == 1.f;
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
         top[k] = x[k][0];
 #pragma unroll
         for (int i = 1; i < 2 * KB; ++i) top[k] = fmaxf(top[k], x[k][i]);
-        grow |= !(ex2_approx(fmaf(top[k], cq[k], -ref[k])) * step <= 65000.f);
+        grow |= !(fmaf(top[k], cq[k], -ref[k]) <= __uint_as_float(bounds[1]));
       }
+      bool wide = false;
       if (__any_sync(0xffffffffu, grow)) {
-        float widest = 0x1p-90f;  // of all lanes; a NaN step does not count
+        const int was_w = window_s[warp];
+        int now = was_w;
+        if (__any_sync(0xffffffffu, off)) {  // the tile's window; NaN groups do not count
+          int s_max = 0, m_max = 0;
 #pragma unroll
-        for (int i = 0; i < 2 * KB; ++i)
-#pragma unroll
-          for (int j = 0; j < NG; ++j) widest = fmaxf(widest, kv4_step(pv[i][j]));
-        const float room =
-            12.f - float(int(__reduce_max_sync(0xffffffffu, __float_as_uint(widest)) >> 23) - 126);
+          for (int i = 0; i < C::WPL; ++i) {
+            const int s = pw[i] & 0x7fff, m = pw[i] >> 16 & 0x7fff;
+            if (s >= 0x7f80 || (lane * C::WPL + i) / NG >= valid) continue;
+            s_max = max(s_max, s), m_max = max(m_max, m);
+          }
+          s_max = __reduce_max_sync(0xffffffffu, s_max);
+          m_max = __reduce_max_sync(0xffffffffu, m_max);
+          if (was_w != kNoWindow) now = fit_window(was_w, s_max, m_max);
+          wide = now == kNoWindow;
+          set_window(now, !wide);
+        }
+        // (of wide mode: p of at most 1)
+        auto room_of = [](int w) { return w == kNoWindow ? 0.f : float(12 + 127 - (w >> 7)); };
+        const float room = room_of(now), was_room = room_of(was_w);
 #pragma unroll
         for (int k = 0; k < NC; ++k)
 #pragma unroll
@@ -676,6 +843,9 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
             go_far();
           }
         }
+        float shift[NC];  // log2 of what the sums so far are multiplied by
+#pragma unroll
+        for (int k = 0; k < NC; ++k) shift[k] = 0.f;
         if (cq[0] == 1.f) {
 #pragma unroll
           for (int k = 0; k < NC; ++k) {
@@ -686,14 +856,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
             top[k] = e(top[k]);
             const float M = fmaxf(was, top[k]);
             if (M > -INFINITY) {
-              const float f = ex2_approx(was - M);
-              l[k] *= f;
-#pragma unroll
-              for (int j = 0; j < NG; ++j) {
-                cm[k][j] *= f;
-#pragma unroll
-                for (int i = 0; i < OD; ++i) o[k][j][i] *= f;
-              }
+              shift[k] = was - M;
 #pragma unroll
               for (int i = 0; i < 2 * KB; ++i) x[k][i] = e(x[k][i]) - M;
               top[k] -= M;
@@ -703,74 +866,109 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
             __syncwarp();
           }
         }
+        // ref moves with the window and grows, in whole numbers, so that the sums
+        // move by powers of two
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
-          const float r = fmaxf(ref[k], fmaf(top[k], cq[k], -room)), al = ex2_approx(ref[k] - r);
+          const float r = fmaxf(ref[k] + (was_room - room), ceilf(top[k] * cq[k]) - room);
+          shift[k] += ref[k] - r;
           ref[k] = r;
-          l[k] *= al;
+        }
+        if (wide) {
+          Wide<D, NC> w;
 #pragma unroll
-          for (int j = 0; j < NG; ++j) {
-            cm[k][j] *= al;
+          for (int k = 0; k < NC; ++k) {
 #pragma unroll
-            for (int i = 0; i < OD; ++i) o[k][j][i] *= al;
+            for (int i = 0; i < 2 * KB; ++i) w.x[k][i] = x[k][i];
+            w.cq[k] = cq[k], w.ref[k] = ref[k], w.l[k] = l[k], w.shift[k] = shift[k];
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+              w.cm[k][j] = cm[k][j];
+              cm[k][j] = 0.f;
+#pragma unroll
+              for (int i = 0; i < OD; ++i) w.o[k][j][i] = o[k][j][i];
+            }
+          }
+          wide_tile<D, NC>(w, unit_s[warp], base, valid, was_w != kNoWindow);
+#pragma unroll
+          for (int k = 0; k < NC; ++k) {
+            l[k] = w.l[k];
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+#pragma unroll
+              for (int i = 0; i < OD; ++i) o[k][j][i] = w.o[k][j][i];
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < NC; ++k) {
+            const float al = ex2_approx(shift[k]);
+            l[k] *= al;
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+              cm[k][j] *= al;
+#pragma unroll
+              for (int i = 0; i < OD; ++i) o[k][j][i] *= al;
+            }
           }
         }
       }
-#pragma unroll
-      for (int k = 0; k < NC; ++k)
-#pragma unroll
-        for (int i = 0; i < 2 * KB; ++i) {
-          p[k][i] = ex2_approx(fmaf(x[k][i], cq[k], -ref[k]));
-          l[k] += p[k][i];
-        }
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        uint32_t pb[NC][2 * KB];
-#pragma unroll
-        for (int i = 0; i < 2 * KB; ++i) {
-          const float s = kv4_step(pv[i][j]), c8 = fmaf(8.f, s, kv4_min(pv[i][j]));
-#pragma unroll
-          for (int k = 0; k < NC; ++k) {
-            cm[k][j] = fmaf(p[k][i], c8, cm[k][j]);
-            pb[k][i] = transpose8(two_parts(p[k][i] * s));
-          }
-        }
-        float c[NC][2][4] = {};
-        uint32_t w[4];
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-          // the codes of 4 dims of positions 16 b + 2 t, + 1 (u) and + 8, + 9 (v)
-          uint32_t u, v;
-          if constexpr (D == 16) {  // byte g of the rows
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = lds32(base + C::CODE + (16 * b + 8 * (i >> 1) + 2 * t + (i & 1)) * 8 +
-                           (g >> 2) * 4);
-            const uint32_t sel = (g & 3) | (4 + (g & 3)) << 8;
-            u = __byte_perm(w[0], w[1], sel);
-            v = __byte_perm(w[2], w[3], sel);
-          } else {
-            if (b % 2 == 0) ldsm_t(base + C::CODE + chunk_off<D>(16 * b + lane, j), w);
-            u = w[b % 2 * 2], v = w[b % 2 * 2 + 1];
-          }
-          const uint32_t a0 = centred_lo(u), a1 = centred_hi(u);
-          const uint32_t a2 = centred_lo(v), a3 = centred_hi(v);
-#pragma unroll
-          for (int k = 0; k < NC; ++k)
-            mma_f16(c[k][0], a0, a1, a2, a3, pb[k][2 * b], pb[k][2 * b + 1]);
-          if constexpr (D > 16) {
-            const uint32_t b0 = centred_lo(u >> 8), b1 = centred_hi(u >> 8);
-            const uint32_t b2 = centred_lo(v >> 8), b3 = centred_hi(v >> 8);
-#pragma unroll
-            for (int k = 0; k < NC; ++k)
-              mma_f16(c[k][1], b0, b1, b2, b3, pb[k][2 * b], pb[k][2 * b + 1]);
-          }
-        }
+      if (!wide) {
 #pragma unroll
         for (int k = 0; k < NC; ++k)
 #pragma unroll
-          for (int i = 0; i < OD; ++i)
-            o[k][j][i] += c[k][i / 2][i % 2 * 2] + c[k][i / 2][i % 2 * 2 + 1];
+          for (int i = 0; i < 2 * KB; ++i) {
+            p[k][i] = ex2_approx(fmaf(x[k][i], cq[k], -ref[k]));
+            l[k] += p[k][i];
+          }
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          uint32_t pb[NC][2 * KB];
+#pragma unroll
+          for (int i = 0; i < 2 * KB; ++i) {
+            const float s = kv4_step(pv[i][j]), c8 = fmaf(8.f, s, kv4_min(pv[i][j]));
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+              cm[k][j] = fmaf(p[k][i], c8, cm[k][j]);
+              pb[k][i] = transpose8(two_parts(p[k][i] * s));
+            }
+          }
+          float c[NC][2][4] = {};
+          uint32_t w[4];
+#pragma unroll
+          for (int b = 0; b < KB; ++b) {
+            // the codes of 4 dims of positions 16 b + 2 t, + 1 (u) and + 8, + 9 (v)
+            uint32_t u, v;
+            if constexpr (D == 16) {  // byte g of the rows
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                w[i] = lds32(base + C::CODE + (16 * b + 8 * (i >> 1) + 2 * t + (i & 1)) * 8 +
+                             (g >> 2) * 4);
+              const uint32_t sel = (g & 3) | (4 + (g & 3)) << 8;
+              u = __byte_perm(w[0], w[1], sel);
+              v = __byte_perm(w[2], w[3], sel);
+            } else {
+              if (b % 2 == 0) ldsm_t(base + C::CODE + chunk_off<D>(16 * b + lane, j), w);
+              u = w[b % 2 * 2], v = w[b % 2 * 2 + 1];
+            }
+            const uint32_t a0 = centred_lo(u), a1 = centred_hi(u);
+            const uint32_t a2 = centred_lo(v), a3 = centred_hi(v);
+#pragma unroll
+            for (int k = 0; k < NC; ++k)
+              mma_f16(c[k][0], a0, a1, a2, a3, pb[k][2 * b], pb[k][2 * b + 1]);
+            if constexpr (D > 16) {
+              const uint32_t b0 = centred_lo(u >> 8), b1 = centred_hi(u >> 8);
+              const uint32_t b2 = centred_lo(v >> 8), b3 = centred_hi(v >> 8);
+#pragma unroll
+              for (int k = 0; k < NC; ++k)
+                mma_f16(c[k][1], b0, b1, b2, b3, pb[k][2 * b], pb[k][2 * b + 1]);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < NC; ++k)
+#pragma unroll
+            for (int i = 0; i < OD; ++i)
+              o[k][j][i] += c[k][i / 2][i % 2 * 2] + c[k][i / 2][i % 2 * 2 + 1];
+        }
       }
 
       // the stage is read: fetch the tile NST ahead into it
@@ -840,8 +1038,9 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
       // lanes as slots: their reference points and sums
       const bool on = run >> lane & 1;
       const float rs = on ? slot(lane)[HB * D + h] : -INFINITY;
-      const float r = warp_max(rs), f = on ? ex2_approx(rs - r) : 0.f;
-      const float ls = warp_sum(on ? f * slot(lane)[HB * D + HB + h] : 0.f);
+      const float r = warp_max(rs);
+      const float fl = on ? ex2_approx(rs - r) * slot(lane)[HB * D + HB + h] : 0.f;
+      const float ls = warp_sum(fl), f = fl * rcp_approx(ls);
       constexpr int Q = (D + 31) / 32;
       float acc[Q] = {};
       // each warp from the run's first to its last has one of its slots, or none
@@ -859,7 +1058,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
 #pragma unroll
       for (int q = 0; q < Q; ++q)
         if (q * 32 + lane < D) {
-          if (complete) out[h * D + q * 32 + lane] = acc[q] / ls;
+          if (complete) out[h * D + q * 32 + lane] = acc[q];
           else part[h * D + q * 32 + lane] = acc[q];
         }
       if (!complete && lane == 0) part[HB * D + h] = r, part[HB * D + HB + h] = ls;
@@ -879,9 +1078,8 @@ __global__ void __launch_bounds__(kJoinThreads) attn_kv4_join_kernel(const Plan 
   constexpr int HB = C::HB, ITEMS = HB * D / 4;
   constexpr int SL = kJoinThreads / ITEMS;  // 2 or more
   constexpr int PF = 4;                      // loads of the partials that do not wait for the weights
-  extern __shared__ float fac[];  // [partial][HB] weights
+  extern __shared__ float fac[];  // [partial][HB] reference points, then weights; then sums
   __shared__ int sums[2][kJoinThreads / 32], at_s[3];
-  __shared__ float lsum[HB];
   __shared__ float4 acc_s[kJoinThreads];
   const AttnKv4Args& a = pl.a;
   const int VH = pl.VH, M = a.kv.M, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -990,6 +1188,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_kv4_join_kernel(const Plan 
         const int i = base + 32 * u;
         if (i >= nb) break;
         fac[i * HB + warp] = x[u];
+        fac[(nb + i) * HB + warp] = l[u];
         // (the sum so far moves with the reference point)
         const float n = fmaxf(r, x[u]);
         ls = fmaf(ls, ex2_approx(r - n), l[u] * ex2_approx(x[u] - n));
@@ -997,10 +1196,10 @@ __global__ void __launch_bounds__(kJoinThreads) attn_kv4_join_kernel(const Plan 
       }
     }
     const float top = warp_max(r);
-    ls = warp_sum(lane < nb ? ls * ex2_approx(r - top) : 0.f);
+    const float f = rcp_approx(warp_sum(lane < nb ? ls * ex2_approx(r - top) : 0.f));
 #pragma unroll 1
-    for (int i = lane; i < nb; i += 32) fac[i * HB + warp] = ex2_approx(fac[i * HB + warp] - top);
-    if (lane == 0) lsum[warp] = ls;
+    for (int i = lane; i < nb; i += 32)
+      fac[i * HB + warp] = ex2_approx(fac[i * HB + warp] - top) * fac[(nb + i) * HB + warp] * f;
   }
   __syncthreads();
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1027,8 +1226,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_kv4_join_kernel(const Plan 
       const float4 o = acc_s[s * ITEMS + tid];
       acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
     }
-    const float f = 1.0f / lsum[h];
-    reinterpret_cast<float4*>(out)[it] = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+    reinterpret_cast<float4*>(out)[it] = acc;
   }
 }
 
@@ -1111,10 +1309,10 @@ cudaError_t run(const AttnKv4Args& a, cudaStream_t s) {
   // Streams of up to 300 positions, 8 heads of 64, all in all: 800 head groups 20.3
   // us with a CTA each and 20.1 by main CTAs, 2048: 33.3 and 27.8, 8192: 91 and 57;
   // 192: 11.2 and 12.2
+  const int fac = 2 * grid * C::HB * 4;
   if (groups > 4 * grid)
-    return launch(attn_kv4_join_kernel<D, NC, true>, grid, kJoinThreads, grid * C::HB * 4, s, pl, grid);
-  return launch(attn_kv4_join_kernel<D, NC, false>, int(groups), kJoinThreads, grid * C::HB * 4, s, pl,
-                grid);
+    return launch(attn_kv4_join_kernel<D, NC, true>, grid, kJoinThreads, fac, s, pl, grid);
+  return launch(attn_kv4_join_kernel<D, NC, false>, int(groups), kJoinThreads, fac, s, pl, grid);
 }
 
 template <int D, int NC>
