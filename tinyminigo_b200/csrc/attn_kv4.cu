@@ -193,20 +193,27 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 __device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
 
-// A head group's window: a power of two 2^K, as its bf16 pattern (K + 127) << 7, such
-// that the steps s and minima m of its values so far have s <= 2^K, |m| <= 2^(K +
-// kMinima), K from kLeast to kFar.  Weights are scaled so that p 2^K is at most 2^16, thus p s
-// fits f16; sums of p |m| stay below 2^(16 + 36) a position, those of p below 2^106.
-constexpr int kMinima = 36, kLeast = -90, kFar = 20;
+// A tile's window: a power of two 2^K, as its bf16 pattern (K + 127) << 7, such
+// that every step s and minimum m of the tile's values has
+//   max(s, |m| / 8) >= 2^(K - kDepth),  s <= 2^K,  |m| <= 2^(K + kMinima)
+// (a group of zeros aside, see the kernel), K within +-kFar.  Weights are scaled so
+// that p 2^K is at most 2^16, thus p s fits f16, and 2^11 at least for the largest
+// weight when it comes, where p max(s, |m| / 8) is then 2^-1: what the two f16 parts
+// of p s leave out of a position (2^-25, times codes of up to 8) is as small beside
+// that as a rounding of f32.  Sums of p |m| over up to 2^31 positions stay below
+// 2^(16 + 36 + 31), and moved to another window (by 2^40) below 2^123.
+constexpr int kDepth = 12, kMinima = 36, kFar = 20;
 constexpr int kNoWindow = 0x7fff;  // no value passes it
 __device__ __forceinline__ int window_of(int K) { return (K + 127) << 7; }
-// The window that steps up to s_max and minima up to m_max (as bf16 patterns) fit:
-// `now` if it does, else one with some room for larger steps.
-__device__ __forceinline__ int fit_window(int now, int s_max, int m_max) {
-  if (s_max <= now && m_max <= now + (kMinima << 7)) return now;
+// The window that steps up to s_max, minima up to m_max and a least max(s, |m| / 8)
+// of `low` fit (all as bf16 patterns; without any, s_max = m_max = 0 and low =
+// 0x7f80): `now` if it does, else one with some room for larger steps.
+__device__ __forceinline__ int fit_window(int now, int s_max, int m_max, int low) {
+  if (s_max <= now && m_max <= now + (kMinima << 7) && low >= now - (kDepth << 7)) return now;
   const int least = max(max((s_max + 0x7f) & ~0x7f, ((m_max + 0x7f) & ~0x7f) - (kMinima << 7)),
-                        window_of(kLeast));
-  return least <= window_of(kFar) ? min(least + (3 << 7), window_of(kFar)) : kNoWindow;
+                        window_of(-kFar));
+  const int most = min((low & ~0x7f) + (kDepth << 7), window_of(kFar));
+  return least <= most ? min(least + (3 << 7), most) : kNoWindow;
 }
 
 // The tiles of all streams, in order of (stream, head group, tile).
@@ -348,9 +355,10 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
   __shared__ int pre[kKv4MaxStreams + 1];  // tiles before each stream
   __shared__ int scan_s[kWarps];
   __shared__ float far_s[kWarps][2][HB];
-  // a head group's window as bounds (set_window), and as it is
-  __shared__ __align__(16) uint32_t bounds_s[kWarps][2];
-  __shared__ int window_s[kWarps];
+  // a head group's window as two bounds (set_window), and as it is; the groups of zeros
+  // and others that it has had
+  __shared__ __align__(16) uint32_t bounds_s[kWarps][4];
+  __shared__ int window_s[kWarps][2];
   __shared__ int unit_s[kWarps][HB][NG];  // exponents of o (wide mode)
   __shared__ int slot_seg[2 * kWarps];  // head group of each warp's partials, -1: none
   const AttnKv4Args& a = pl.a;
@@ -538,14 +546,16 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
     }
     __syncwarp();
   };
-  // The head group's window, and whether the next tile is tested against it (else it is off).
-  auto set_window = [&](int now, bool test) {
-    const int w = test ? now : kNoWindow;
+  // The head group's window; that which the next tile is tested against (none: always
+  // off); its groups of zeros (bits 0-3) and others (4-7).
+  auto set_window = [&](int now, int test, unsigned zn) {
     __syncwarp();
     if (lane == 0) {
-      bounds_s[warp][0] = w * 0x10001u + (kMinima << 23);
-      bounds_s[warp][1] = __float_as_uint(w == kNoWindow ? -INFINITY : 15.98f + 127 - (w >> 7));
-      window_s[warp] = now;
+      bounds_s[warp][0] = test * 0x10001u + (kMinima << 23);
+      bounds_s[warp][1] = 0x80000000u | (test - (kDepth << 7));
+      bounds_s[warp][2] =
+          __float_as_uint(test == kNoWindow ? -INFINITY : 15.98f + 127 - (test >> 7));
+      window_s[warp][0] = now, window_s[warp][1] = zn;
     }
     __syncwarp();
   };
@@ -600,7 +610,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
         for (int i = 0; i < OD; ++i) o[k][j][i] = 0.f;
       }
     }
-    set_window(window_of(kLeast), false);
+    set_window(window_of(0), window_of(0), 0);  // a first guess, for values of ordinary size
     bool over = false;
 #pragma unroll
     for (int k = 0; k < NC; ++k) over |= cq[k] >= 0x1p100f;
@@ -615,7 +625,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
   // becomes the weighted mean of the values, which f32 holds whatever they are
   auto finish = [&]() {
     __syncwarp();
-    const bool wide = window_s[warp] == kNoWindow;
+    const bool wide = window_s[warp][0] == kNoWindow;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
 #pragma unroll
@@ -769,8 +779,8 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
       // a share of them: word i is of position (lane WPL + i) / NG, group i % NG
       uint32_t pw[C::WPL];
       lds_words<C::WPL>(base + 2 * C::CODE + C::PAR + lane * C::WPL * 4, pw);
-      uint32_t bounds[2];
-      lds_words<2>(smem_u32(bounds_s[warp]), bounds);
+      uint32_t bounds[4];
+      lds_words<4>(smem_u32(bounds_s[warp]), bounds);
       if (valid < TK) {
 #pragma unroll
         for (int i = 0; i < 2 * KB; ++i)
@@ -792,11 +802,14 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
       // the largest negative minimum, the signed one the largest positive minimum.  A
       // NaN step is above all.
       uint32_t most = __vmaxu2(pw[0], pw[1]), most_s = __vmaxs2(pw[0], pw[1]);
+      uint32_t least = __vmins2(pw[0], pw[1]);
       if constexpr (C::WPL == 4) {
         most = __vimax3_u16x2(most, pw[2], pw[3]);
         most_s = __vimax3_s16x2(most_s, pw[2], pw[3]);
+        least = __vimin3_s16x2(least, pw[2], pw[3]);
       }
-      const bool off = __vimax3_s16x2(most & 0x7fffffffu, most_s, bounds[0]) != bounds[0];
+      const bool off = __vimax3_s16x2(most & 0x7fffffffu, most_s, bounds[0]) != bounds[0] ||
+                       __vmins2(least, bounds[1]) != bounds[1];
       float p[NC][2 * KB];
       float top[NC];
       bool grow = off || cq[0] == 1.f;
@@ -805,25 +818,37 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
         top[k] = x[k][0];
 #pragma unroll
         for (int i = 1; i < 2 * KB; ++i) top[k] = fmaxf(top[k], x[k][i]);
-        grow |= !(fmaf(top[k], cq[k], -ref[k]) <= __uint_as_float(bounds[1]));
+        grow |= !(fmaf(top[k], cq[k], -ref[k]) <= __uint_as_float(bounds[2]));
       }
       bool wide = false;
       if (__any_sync(0xffffffffu, grow)) {
-        const int was_w = window_s[warp];
-        int now = was_w;
-        if (__any_sync(0xffffffffu, off)) {  // the tile's window; NaN groups do not count
-          int s_max = 0, m_max = 0;
+        int was_w = window_s[warp][0], now = was_w;
+        if (__any_sync(0xffffffffu, off)) {
+          // the tile's window (NaN groups do not count), and which of its groups have
+          // zeros (z) or others (n).  A group that has had both has no window: the
+          // zeros may have all the weight that ref counts from.
+          int s_max = 0, m_max = 0, low = 0x7f80;
+          unsigned zn = 0;
 #pragma unroll
           for (int i = 0; i < C::WPL; ++i) {
             const int s = pw[i] & 0x7fff, m = pw[i] >> 16 & 0x7fff;
             if (s >= 0x7f80 || (lane * C::WPL + i) / NG >= valid) continue;
-            s_max = max(s_max, s), m_max = max(m_max, m);
+            const int b = max(s, m - (3 << 7));
+            zn |= (b > 0 ? 16u : 1u) << (i % NG);
+            if (b > 0) s_max = max(s_max, s), m_max = max(m_max, m), low = min(low, b);
           }
           s_max = __reduce_max_sync(0xffffffffu, s_max);
           m_max = __reduce_max_sync(0xffffffffu, m_max);
-          if (was_w != kNoWindow) now = fit_window(was_w, s_max, m_max);
+          low = __reduce_min_sync(0xffffffffu, low);
+          zn = __reduce_or_sync(0xffffffffu, zn) | window_s[warp][1];
+          if (was_w != kNoWindow)
+            now = zn & zn >> 4 & 15u ? kNoWindow : fit_window(was_w, s_max, m_max, low);
           wide = now == kNoWindow;
-          set_window(now, !wide);
+          // (tiles that pass the test later have no group of zeros)
+          if (wide || (zn & 15u)) set_window(now, kNoWindow, zn);
+          else set_window(now, now, 0xf0u);
+        } else if (lane == 0) {
+          window_s[warp][1] = 0xf0;
         }
         // (of wide mode: p of at most 1)
         auto room_of = [](int w) { return w == kNoWindow ? 0.f : float(12 + 127 - (w >> 7)); };
