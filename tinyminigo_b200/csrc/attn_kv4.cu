@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
     int st = 0;
     uint32_t phase = 0;
     for (int T = w0; T < w1; ++T) {
-      if (!mbar_wait(&full[warp][st], phase)) {
+      if (!mbar_wait_warp(&full[warp][st], phase)) {
         if (lane == 0 && a.err) atomicCAS(a.err, 0, 2);
         alive = false;
         break;

@@ -425,9 +425,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       }
       alpha_prev = alpha;
     }
+    ok = __all_sync(0xffffffffu, ok);  // the last block's wait has no barrier behind it
     if (ok) {
       const int i = nb - 1, bi = i & 1;
-      if (!mbar_wait(&o_full[bi], (i >> 1) & 1)) {
+      if (!mbar_wait_warp(&o_full[bi], (i >> 1) & 1)) {
         ok = false;
       } else {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

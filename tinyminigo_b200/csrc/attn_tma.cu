@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kTmaThreads, D == 64 ? 3 : 2)
     for (int i = 0; i < ntiles; ++i) {
       const int s = i % NS;
       const uint32_t ph = (i / NS) & 1;
-      const bool ok = !abort_s && mbar_wait(&full[s], ph);
+      const bool ok = !__any_sync(0xffffffffu, abort_s) && mbar_wait_warp(&full[s], ph);
       if (!ok) {
         if (lane == 0) {
           abort_s = 1;

@@ -123,6 +123,29 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
     }
   }
 }
+// The same by a whole warp, with one outcome for all its lanes.  (By lanes it could
+// end either way near the limit, each keeping its own time, and those that go on
+// would meet the warp's next shuffle or matrix instruction without the others.)
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity) {
+  const uint32_t a = smem_u32(bar);
+  unsigned long long t0 = 0;
+  for (unsigned int i = 0;; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (__all_sync(0xffffffffu, ok)) return true;
+    if ((i & 63) == 0) {
+      const unsigned long long t = global_ns();
+      if (i == 0) t0 = t;
+      if (__any_sync(0xffffffffu, t - t0 > kWaitNs)) return false;
+    }
+  }
+}
 // Non-blocking test: has the phase of parity `parity` completed?
 __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
   uint32_t ok;

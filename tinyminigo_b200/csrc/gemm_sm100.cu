@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     int tl = 0;
     for (int t = blockIdx.x; t < tiles && !failed; t += gridDim.x, ++tl) {
       const int buf = tl & 1;
-      if (!mbar_wait(&acc_full[buf], (tl >> 1) & 1)) {
+      if (!mbar_wait_warp(&acc_full[buf], (tl >> 1) & 1)) {
         atomicExch(a.err, 2);
         failed = 1;
         break;
