@@ -1257,7 +1257,10 @@ int forward_seq(tmg_ctx* c, tmg_kv* kv, int stream, const uint32_t* tokens, int6
 // to the host.
 int score_rows(tmg_ctx* c, const uint32_t* tokens, int64_t t0, int64_t Tc, int64_t T,
                const Scores& out) {
-  const int64_t R = std::min<int64_t>(kScoreRows, c->pf_cap);
+  // room for as many rows as there are (a power of two, so that scoring a little
+  // more each time seldom has to grow it), not for the longest prefill's
+  int64_t R = 1;
+  while (R < std::min(kScoreRows, Tc)) R *= 2;
   const size_t per = 3 + 2 * size_t(out.n_top);  // a row's target, logprob, entropy, alternatives
   const size_t need = size_t(R) * c->V * 4 + size_t(Tc) * per * 4;
   if (c->sc_cap < need) {
