@@ -2484,6 +2484,7 @@ int tmg_fused_group_init(tmg_ctx* c, tmg_kv* kv, const uint8_t id[128], int32_t 
   if (!c || !kv || kv->ctx != c || !id || world < 2 || world > kMaxGroupRanks || rank < 0 ||
       rank >= world)
     return fail(c, TMG_ERR_INVALID, "bad argument");
+  if (kv->q4) return fail(c, TMG_ERR_INVALID, "tmg_fused_group_init does not take a 4-bit cache");
   if (c->world != 1 || !use_fused(c, kv) || kv->grp)
     return fail(c, TMG_ERR_INVALID,
                 "a fused group needs a single-GPU context with full weights whose shape the fused "
