@@ -27,7 +27,7 @@ torch = pytest.importorskip("torch")
 if not torch.cuda.is_available():  # pragma: no cover - CPU box
     pytest.skip("needs a GPU", allow_module_level=True)
 
-from test_gpu_kv4 import attend, dev, filled  # noqa: E402
+from test_gpu_kv4 import Cache, attend, dev, filled  # noqa: E402
 
 from tinyminigo_b200._lib import check, lib  # noqa: E402
 
@@ -56,9 +56,12 @@ def set_values(c, codes=None, params=None, keys=False):
         pp[:params.size] = dev(np.ascontiguousarray(params).reshape(-1).view(np.int32))
 
 
-def compare(ctx, c, q, lens):
-    """The attention against 64 bits, each output within its own tolerance."""
+def compare(ctx, c, q, lens, copies=1):
+    """The attention against 64 bits, each output within its own tolerance; of `copies`
+    of the heads the first, which the others equal."""
     out = attend(ctx, c, q, lens)
+    again = out.reshape(out.shape[0], copies, -1)
+    assert np.array_equal(again, np.broadcast_to(again[:, :1], again.shape))
     (kc, kp), (vc, vp) = c.host()
     M, n_q, d = q.shape
     per = n_q // c.n_kv
@@ -71,7 +74,7 @@ def compare(ctx, c, q, lens):
         v = R.values(vc[m, :, :n], vp[m, :, :n])
         low = R.bf16_value(vp[m, :, :n] >> np.uint32(16)).astype(np.float64)
         b = np.maximum(np.abs(low), np.abs(low + 15.0 * R.steps(vp[m, :, :n])))
-        for h in range(n_q):
+        for h in range(n_q // copies):
             kv = h // per
             x = k[kv] @ q[m, h].astype(np.float64) / np.sqrt(d)
             A = (np.abs(k[kv]) @ np.abs(q[m, h].astype(np.float64))).max() / np.sqrt(d)
@@ -134,11 +137,11 @@ def along(rng, n_kv, group, d):
     return q.reshape(1, n_kv * group, d).astype(np.float32), way
 
 
-def put(rng, d, n, n_kv, group, values, scores=None):
+def put(rng, d, n, n_kv, group, values, scores=None, copies=1):
     """A cache of n positions with the values [1, n_kv, n, d]; keys of size 1, at the
-    positions of `scores` along the queries, and the queries."""
+    positions of `scores` along the queries, and the queries.  All of it `copies` times."""
     cap = (n + 3) // 4 * 4
-    c = filled(rng, 1, n_kv, d, cap, [n])
+    c = Cache(1, n_kv * copies, d, cap)
     q, way = along(rng, n_kv, group, d)
     k = rng.normal(0, 0.3, (1, n_kv, cap, d))
     for at, x in (scores or {}).items():
@@ -148,8 +151,8 @@ def put(rng, d, n, n_kv, group, values, scores=None):
     for part, keys in ((k, True), (x, False)):
         codes, params = R.quantise(part.astype(np.float32))
         params[:, :, n:] = 0x7FC07FC0
-        set_values(c, codes, params, keys)
-    return c, q
+        set_values(c, np.tile(codes, (1, copies, 1, 1)), np.tile(params, (1, copies, 1, 1)), keys)
+    return c, np.tile(q, (1, copies, 1))
 
 
 @pytest.mark.parametrize("d", [16, 32, 64, 128])
@@ -275,3 +278,38 @@ def test_nan_groups_stay_in_their_columns(ctx):
         assert np.isnan(out[0, 4:, 32:]).all()
         assert not np.isnan(out[0, 4:, :32]).any() and not np.isnan(out[0, :4]).any()
     assert np.isfinite(clean).all()
+
+
+@pytest.mark.parametrize("d,group", [(16, 4), (32, 9), (64, 4), (128, 4), (128, 8)])
+@pytest.mark.parametrize("base,e,score", [(0, 12, -15.0), (-15, 30, -25.0), (-15, 34, -30.0),
+                                          (-18, 15, -12.0), (3, 17, -14.0)])
+def test_a_wide_stretch_of_little_weight(ctx, d, group, base, e, score):
+    # whole tiles of positions 2^e wider than those before and behind, each with so
+    # much less weight that they make up about as much of the result.  So many head
+    # groups that each stays on one SM: a warp takes 4 tiles (of 64 positions, of 32
+    # for heads of 128) in a row.
+    rng = np.random.default_rng(d + e)
+    tile, copies = 32 if d == 128 else 64, 40 if group <= 8 else 20
+    n = 64 * tile
+    at = np.arange(n) // tile % 4 // 2 == 1 if e % 2 else np.arange(n) // tile % 4 == 1
+    v = rng.normal(0, 2.0 ** base, (1, 2, n, d))
+    v[0, :, at] *= 2.0 ** e
+    c, q = put(rng, d, n, 2, group, v, {int(i): score for i in np.flatnonzero(at)}, copies)
+    compare(ctx, c, q, [n], copies)
+
+
+@pytest.mark.parametrize("d,group", [(16, 4), (64, 4), (64, 9), (128, 4)])
+@pytest.mark.parametrize("e", [-30, -8, 8, 14, 30, 50])
+def test_sizes_that_change_on_the_way(ctx, d, group, e):
+    # stretches of one size, the other, constants and zeros, in a row of one warp
+    rng = np.random.default_rng(d + abs(e))
+    tile, copies = 32 if d == 128 else 64, 40 if group <= 8 else 20
+    n = 64 * tile
+    v = rng.normal(0, 1, (1, 2, n, d))
+    kind = np.arange(n) // (tile // 2 + 5) % 11
+    v[:, :, kind == 3] *= 2.0 ** e
+    v[:, :, kind == 5] = 2.0 ** e
+    v[:, :, kind == 8] *= 2.0 ** -e
+    v[:, 1, kind == 9] = 0.0
+    c, q = put(rng, d, n, 2, group, v, copies=copies)
+    compare(ctx, c, q, [n], copies)

@@ -207,12 +207,12 @@ constexpr int kNoWindow = 0x7fff;  // no value passes it
 __device__ __forceinline__ int window_of(int K) { return (K + 127) << 7; }
 // The window that steps up to s_max, minima up to m_max and a least max(s, |m| / 8)
 // of `low` fit (all as bf16 patterns; without any, s_max = m_max = 0 and low =
-// 0x7f80): `now` if it does, else one with some room for larger steps.
-__device__ __forceinline__ int fit_window(int now, int s_max, int m_max, int low) {
+// 0x7f80): `now` if it does, else one with some room for larger steps, `cap` at most.
+__device__ __forceinline__ int fit_window(int now, int cap, int s_max, int m_max, int low) {
   if (s_max <= now && m_max <= now + (kMinima << 7) && low >= now - (kDepth << 7)) return now;
   const int least = max(max((s_max + 0x7f) & ~0x7f, ((m_max + 0x7f) & ~0x7f) - (kMinima << 7)),
                         window_of(-kFar));
-  const int most = min((low & ~0x7f) + (kDepth << 7), window_of(kFar));
+  const int most = min((low & ~0x7f) + (kDepth << 7), cap);
   return least <= most ? min(least + (3 << 7), most) : kNoWindow;
 }
 
@@ -251,10 +251,12 @@ struct Cursor {
 };
 
 // Wide mode: values that no window holds (steps or minima of one tile far apart,
-// or near the ends of f32).  From there on to the head group's end p is at most 1,
-// cm is 0 and o counts in units of 2^unit[head][group], a bound of p |v| so far, to
+// near the ends of f32, or much larger than those before).  There p is at most 1, cm
+// is 0 and o counts in units of 2^unit[head][group], a bound of p |v| so far, to
 // which each product goes as a 64-bit number; so it is as exact as 32-bit sums, and
-// neither |v| nor what p leaves of it can leave f32.  A function of its own, called
+// neither |v| nor what p leaves of it can leave f32.  A tile takes some 10 times as
+// long so (all of 16 x 32768: 804 us).  It ends with a tile whose window holds what
+// the sums hold, too.  A function of its own, called
 // for such tiles only: in the loop its registers would cost every tile (8 heads of
 // 128 a kv head: 130 us and not 115).
 template <int D, int NC>
@@ -825,8 +827,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
         int was_w = window_s[warp][0], now = was_w;
         if (__any_sync(0xffffffffu, off)) {
           // the tile's window (NaN groups do not count), and which of its groups have
-          // zeros (z) or others (n).  A group that has had both has no window: the
-          // zeros may have all the weight that ref counts from.
+          // zeros (z) or others (n)
           int s_max = 0, m_max = 0, low = 0x7f80;
           unsigned zn = 0;
 #pragma unroll
@@ -837,13 +838,48 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
             zn |= (b > 0 ? 16u : 1u) << (i % NG);
             if (b > 0) s_max = max(s_max, s), m_max = max(m_max, m), low = min(low, b);
           }
+          zn = __reduce_or_sync(0xffffffffu, zn);
+          unsigned had = window_s[warp][1];
+          int cap = window_of(kFar);
+          if (was_w != kNoWindow) {
+            // What the tiles before hold is 2^(K - kDepth) at least, by their window, so
+            // it may fall but not rise (but before the first).
+            if (had) cap = was_w;
+          } else {
+            // What the sums hold by now: 2^(e - 1) at least, max(s, |m| / 8) being a
+            // quarter of b or more.
+            had = 0;
+#pragma unroll
+            for (int k = 0; k < NC; ++k)
+#pragma unroll
+              for (int j = 0; j < NG; ++j) {
+                const int e = unit_s[warp][4 * k + t][j];
+                if (e == -4000 && (zn >> j & 0x11u) == 1u) continue;  // zeros, and still
+                had |= 16u << j;
+                low = min(low, max(e - 3 + 127, 0) << 7);
+                m_max = max(m_max, max(e + 127, 0) << 7);
+              }
+            had = __reduce_or_sync(0xffffffffu, had);
+          }
           s_max = __reduce_max_sync(0xffffffffu, s_max);
           m_max = __reduce_max_sync(0xffffffffu, m_max);
           low = __reduce_min_sync(0xffffffffu, low);
-          zn = __reduce_or_sync(0xffffffffu, zn) | window_s[warp][1];
-          if (was_w != kNoWindow)
-            now = zn & zn >> 4 & 15u ? kNoWindow : fit_window(was_w, s_max, m_max, low);
+          // A group with zeros and others has no window: the zeros may have all the
+          // weight that ref counts from.
+          zn |= had;
+          now = zn & zn >> 4 & 15u ? kNoWindow : fit_window(was_w, cap, s_max, m_max, low);
           wide = now == kNoWindow;
+          if (was_w == kNoWindow && !wide) {  // o as other tiles have it
+#pragma unroll
+            for (int k = 0; k < NC; ++k)
+#pragma unroll
+              for (int j = 0; j < NG; ++j) {
+                const float f =
+                    __int_as_float((max(unit_s[warp][4 * k + t][j], -126) + 127) << 23);
+#pragma unroll
+                for (int i = 0; i < OD; ++i) o[k][j][i] *= f;
+              }
+          }
           // (tiles that pass the test later have no group of zeros)
           if (wide || (zn & 15u)) set_window(now, kNoWindow, zn);
           else set_window(now, now, 0xf0u);
