@@ -160,7 +160,10 @@ int tmg_kv_create(tmg_ctx* ctx, int32_t n_streams, int64_t capacity, tmg_kv** ou
  * too, sees the rows as the cache holds them, so logits do not depend on how a
  * prompt is cut into calls beyond rounding.  Takes every call that a tmg_kv
  * does except tmg_fused_group_init and the trace aids; greedy decode runs the
- * per-step graph.  One layer and stream of f32 rows is kept beside it for
+ * per-step graph, not the fused kernel that one stream of f32 rows takes, so it
+ * is the faster one for long contexts only (1B-class model, one stream: 1.05 ms a
+ * token at 512 positions where f32 rows take 0.65, even at about 8000, 1.21 and
+ * 2.65 at 32768).  One layer and stream of f32 rows is kept beside it for
  * prefill.  head_dim 16, 32, 64 or 128, at most 16 query heads per kv head. */
 int tmg_kv_create_q4(tmg_ctx* ctx, int32_t n_streams, int64_t capacity, tmg_kv** out);
 int tmg_kv_destroy(tmg_kv* kv);
@@ -443,7 +446,11 @@ int tmg_op_kv4_read(tmg_ctx* ctx, const tmg_kv4* kv, const int32_t* pos, const i
  * each stream m one query row q + m * q_ld of n_q heads over its first
  * lens[m] positions, to out + m * out_ld (a stream of length 0 gets zeros;
  * out may be q, with the same leading dimension).
- * At most 16 query heads per kv head.  max_len: a bound of all lengths that
+ * At most 16 query heads per kv head.  Sums are held in f32, queries to 22 bits
+ * and to 2^-35 of their head's largest element.  Values may have any size that
+ * the format holds; where their steps differ by more than 2^12 within 32 or 64
+ * neighbouring positions, or lie outside 2^-32 to 2^20, those positions take
+ * about ten times as long.  max_len: a bound of all lengths that
  * the caller knows (the capacity if none), which sizes the split; a length
  * outside [0, max_len] is taken as the nearer end (TMG_ERR_INVALID).  ws: at
  * least the bytes that tmg_op_attn_decode_kv4_ws reports, 16-byte aligned,

@@ -51,7 +51,8 @@ def parse_args(argv=None) -> argparse.Namespace:
     ap.add_argument("--seed", metavar="SEED", type=int, default=42,
                     help="Random seed for sampling")
     ap.add_argument("--kv-bits", metavar="B", type=int, default=32, choices=(4, 32),
-                    help="Bits of a KV cache element: 32, or 4 (not in the reference)")
+                    help="Bits of a KV cache element: 32, or 4 (not in the reference; slower "
+                         "than 32 for short contexts, below about 8000 tokens of a 1B model)")
     ap.add_argument("prompt", help="The user prompt")
     ap.add_argument("--dump-first-logits", metavar="FILE", default=None,
                     help=argparse.SUPPRESS)

@@ -7,30 +7,35 @@
 // s), q . k_t = sum over groups of s (q . c) + m (sum of q): the products
 // with codes are exact 4-bit integers times q, which the warp matrix
 // instruction takes as f16, and s and m are applied to 32-bit sums.  q is
-// carried as two f16 parts (22 bits; scaled per head by a power of two so
-// that neither part leaves f16's range), the parts as neighbouring columns of
-// one instruction.  Likewise o = sum_t (p_t s_t) (c_t - 8) + sum_t p_t (m_t +
-// 8 s_t): p s in two f16 parts; the codes centred, since the sums of c and
-// of m alone are hundreds of times larger than their sum over a long row.
+// carried as two f16 parts (22 bits, and 2^-35 of the head's largest element at
+// least; scaled per head by a power of two so that neither part leaves f16's
+// range), the parts as neighbouring columns of one instruction.  Likewise o =
+// sum_t (p_t s_t) (c_t - 8) + sum_t p_t (m_t + 8 s_t): p s in two f16 parts; the
+// codes centred, since the sums of c and of m alone are hundreds of times larger
+// than their sum over a long row.  p is scaled for the sizes of s and m (windows,
+// below); values that no such scale serves are summed another way (wide_tile).
 //
 // What bounds it: at 5 bits an element the memory brings 37 elements a clock
 // and SM, so 3.4 lane-instructions an element are all there are; a tile of 64
-// positions x 64 (keys and values) takes about 730, 2.9 an element, and the
-// schedulers issue in 63 of 100 clocks (with the fixed parts; the loop in 73).
-// 16 streams of 32768 positions (32 / 8 heads of 64, 336 MB) take 72 us, 4.7
-// TB/s, and 79 in a long run at the power cap's clocks; with the arithmetic
-// left out 61 us where the whole took 78, and the bytes alone are 51.  One
-// stream of 131072 positions takes 26 us for 12.8 of bytes: the list's scan
-// and the first tiles 3.5 us, the joins 5.  The matrix instructions are
-// mma.sync (m16n8k16): a key tile meets 4 heads' two parts in 8 columns, so
-// tcgen05's 128-row tiles with operands in shared memory would spend more on
-// writing widened codes than they save; the tensor pipe is busy a fifth of the
-// time.
+// positions x 64 (keys and values) takes about 750, 2.9 an element, and the
+// schedulers issue in 61 of 100 clocks (both with the fixed parts).  16 streams
+// of 32768 positions (32 / 8 heads of 64, 336 MB) take 73 us, 4.6 TB/s, and 77
+// in a long run at the power cap's clocks; with the arithmetic left out 61 us
+// where the whole took 78, and the bytes alone are 51.  One stream of 131072
+// positions takes 26 us for 12.8 of bytes: the list's scan and the first tiles
+// 3.5 us, the joins 5.  The matrix instructions are mma.sync (m16n8k16): a key
+// tile meets 4 heads' two parts in 8 columns, so tcgen05's 128-row tiles with
+// operands in shared memory would spend more on writing widened codes than they
+// save; the tensor pipe is busy a fifth of the time.  With 5 to 8 query heads a
+// kv head (two column tiles) a warp needs up to 254 registers, so an SM has 8
+// warps; 9 to 16 make two head groups, each of which loads and widens its kv
+// head's tiles for itself.
 //
 // Tiles come by bulk copies into a ring of each warp's own, so no warp waits for
-// another before its head group ends.  (By 16-byte cp.async those 61 us are 76.)  All tiles of all streams are one list that the CTAs, and in
-// them the warps, take equal runs of; a head group that several warps share is
-// joined in shared memory, one that several CTAs share by a second kernel.
+// another before its head group ends.  (By 16-byte cp.async those 61 us are 76.)
+// All tiles of all streams are one list that the CTAs, and in them the warps,
+// take equal runs of; a head group that several warps share is joined in shared
+// memory, one that several CTAs share by a second kernel.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <math.h>
@@ -106,10 +111,14 @@ __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t m, uint32_t o) {
   return y;
 }
 // Two codes in bits 0-3 (or 4-7) of the halves of x to f16 c - 8: 0x6400 | c
-// is 1024 + c, 0x6400 | 16 c is 1024 + 16 c; both steps are exact.
+// is 1024 + c, 0x6400 | 16 c is 1024 + 16 c; both steps are exact.  (Kim et al., "Who
+// Says Elephants Can't Run: Bringing Large Scale MoE Models into Cloud Scale
+// Production", 2022, widen integers by such an exponent.)
 __device__ __forceinline__ uint32_t centred_lo(uint32_t x) {
   uint32_t y;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(and_or(x, 0x000f000fu, 0x64006400u)), "r"(0xe408e408u));
+  asm("add.rn.f16x2 %0, %1, %2;"
+      : "=r"(y)
+      : "r"(and_or(x, 0x000f000fu, 0x64006400u)), "r"(0xe408e408u));
   return y;  // - 1032
 }
 __device__ __forceinline__ uint32_t centred_hi(uint32_t x) {
@@ -376,7 +385,9 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
     }
   mbar_fence_init();
   pdl_wait();
-  pdl_trigger();  // the join may start: it reads lens before it waits for this kernel
+  // The join may start.  It reads lens before it waits for this kernel, so the
+  // trigger stays behind the wait: what wrote lens has then ended.
+  pdl_trigger();
 
   auto checked_tiles = [&](int m) {
     const int len = a.lens[m];

@@ -189,7 +189,9 @@ int attn_decode_noalloc(int device, int num_sms, cudaStream_t s, const float* q,
 
 // ---------------------------------------------------------------------------
 // The 4-bit KV cache (kv4.cuh: layout and arithmetic).  These launches are
-// programmatic (PDL): every kernel waits before it touches memory.
+// programmatic (PDL): every kernel waits before it touches memory, but for the
+// attention's join, which reads lens before (the main kernel lets it start only
+// behind its own wait).
 // ---------------------------------------------------------------------------
 // Values of the device error word (1: NaN logits, 2: a bounded wait gave up).
 constexpr int kErrPosition = 3;  // a row's position lies outside the cache

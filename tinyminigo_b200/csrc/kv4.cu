@@ -11,10 +11,12 @@
 //
 // Reading 65536 rows (8 heads of 128: 84 MB of cache, 537 MB of f32) takes 98
 // us, 6.3 TB/s, 96% of a plain copy's rate.  Writing 4000 rows (32.8 MB in, 5.1
-// MB out) takes 13.5 us, where the bytes are 5.8: two waves of blocks that each
-// load, meet the group's extremes by 3 shuffles and store, at 183 instructions
-// a unit of 256 values, are bounded by that chain's latency and the launch.  A
-// few rows (a step of 16 streams) take a launch's time, about 4 us a call.
+// MB out) takes 11.8 us a call in a graph, where the bytes are 5.8: 2000 blocks, of
+// which 592 are resident (4 an SM, at 61 registers a thread), so 3.4 waves at half
+// the warps that an SM holds, each with its own latency of loads, the group's
+// extremes by 2 rounds of shuffles, 183 instructions a unit of 256 values, and
+// stores.  A few rows (a step of 16 streams) take a launch's time, 2.4 us in a graph
+// and about 4 from the host.
 #include <algorithm>
 
 #include "kv4.cuh"
