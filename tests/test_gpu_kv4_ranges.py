@@ -313,3 +313,22 @@ def test_sizes_that_change_on_the_way(ctx, d, group, e):
     v[:, 1, kind == 9] = 0.0
     c, q = put(rng, d, n, 2, group, v, copies=copies)
     compare(ctx, c, q, [n], copies)
+
+
+@pytest.mark.parametrize("d,group", [(16, 4), (64, 4), (64, 9), (128, 4)])
+@pytest.mark.parametrize("scale", [1e-25, 1e-7, 1e-5, 1e-3, 1e3])
+@pytest.mark.parametrize("score", [1e7, 1e12])
+def test_scores_that_go_far_on_the_way(ctx, d, group, scale, score):
+    # ordinary scores, and in the third tile of a warp one beyond all others: its
+    # values come back, whatever their size
+    rng = np.random.default_rng(d + group)
+    tile, copies = 32 if d == 128 else 64, 40 if group <= 8 else 20
+    n = 64 * tile
+    at = 10 * tile + 5
+    c, q = put(rng, d, n, 2, group, rng.normal(0, scale, (1, 2, n, d)), {at: score}, copies)
+    (_, _), (vc, vp) = c.host()
+    want = R.values(vc[0, :, at], vp[0, :, at])
+    low = R.bf16_value(vp[0, :, at] >> np.uint32(16)).astype(np.float64)
+    b = np.repeat(np.maximum(np.abs(low), np.abs(low + 15.0 * R.steps(vp[0, :, at]))), c.g, -1)
+    out = attend(ctx, c, q, [n])[0].reshape(2 * copies, group, d)
+    assert np.all(np.abs(out - want[:, None]) <= 64 * 2.0 ** -24 * b[:, None])

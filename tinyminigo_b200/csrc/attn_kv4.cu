@@ -548,13 +548,13 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
   // to the head group's end x holds e - M, e the rounded exponent and M the
   // largest so far, cq is 1 (which a product with log2 e never is) and ref
   // counts from M.  cq (without its 2^24) and M of head h: far_s[warp][..][h].
-  auto go_far = [&]() {
+  auto go_far = [&](float room) {
     __syncwarp();
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       far_s[warp][0][4 * k + t] = cq[k];
-      far_s[warp][1][4 * k + t] = ref[k];
-      if (ref[k] > -INFINITY) ref[k] = 0.f;
+      far_s[warp][1][4 * k + t] = ref[k] + room;
+      if (ref[k] > -INFINITY) ref[k] = -room;
       cq[k] = 1.f;
     }
     __syncwarp();
@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
 #pragma unroll
     for (int k = 0; k < NC; ++k) over |= cq[k] >= 0x1p100f;
     if (__any_sync(0xffffffffu, over)) {
-      go_far();
+      go_far(0.f);
     } else {
 #pragma unroll
       for (int k = 0; k < NC; ++k) cq[k] *= 0x1p24f;
@@ -912,7 +912,7 @@ __global__ void __launch_bounds__(Cfg<D, NC>::W * 32, 1)
           if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
             for (int k = 0; k < NC; ++k) cq[k] *= 0x1p-24f;
-            go_far();
+            go_far(was_room);
           }
         }
         float shift[NC];  // log2 of what the sums so far are multiplied by
