@@ -19,8 +19,8 @@
 // and SM, so 3.4 lane-instructions an element are all there are; a tile of 64
 // positions x 64 (keys and values) takes about 750, 2.9 an element, and the
 // schedulers issue in 61 of 100 clocks (both with the fixed parts).  16 streams
-// of 32768 positions (32 / 8 heads of 64, 336 MB) take 73 us, 4.6 TB/s, and 77
-// in a long run at the power cap's clocks; with the arithmetic left out 61 us
+// of 32768 positions (32 / 8 heads of 64, 336 MB) take 73 us, 4.6 TB/s, and 77 to
+// 81 in a long run at the power cap's clocks; with the arithmetic left out 61 us
 // where the whole took 78, and the bytes alone are 51.  One stream of 131072
 // positions takes 26 us for 12.8 of bytes: the list's scan and the first tiles
 // 3.5 us, the joins 5.  The matrix instructions are mma.sync (m16n8k16): a key
